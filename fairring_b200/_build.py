@@ -30,6 +30,7 @@ SOURCES = [
     "emulate.cpp",
     "bench_client.cpp",
     "local_ops.cpp",
+    "logits_ops.cpp",
     "selftest.cpp",
     "kernels/collectives.cu",
     "kernels/collectives_u8.cu",
@@ -45,6 +46,8 @@ SOURCES = [
     "kernels/local_ops.cu",
     "kernels/layernorm.cu",
     "kernels/cross_entropy.cu",
+    "kernels/token_log_probs.cu",
+    "kernels/distillation.cu",
     "kernels/batchnorm.cu",
     "kernels/maxpool.cu",
     "kernels/stem.cu",

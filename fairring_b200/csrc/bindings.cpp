@@ -13,6 +13,7 @@
 #include "backend.h"
 #include "bench_client.h"
 #include "local_ops.h"
+#include "logits_ops.h"
 #include "store_adapter.h"
 
 #include <execinfo.h>
@@ -233,5 +234,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("VEC_BYTES") = kVecBytes;
 
   bindLocalOps(m);
+  bindLogitsOps(m);
   bindSelfTest(m);
 }

@@ -138,6 +138,69 @@ cudaError_t launchEmbedBackward(const float* dx, const int64_t* tokens, float* d
 cudaError_t launchStemFold(const void* image, bool bf16, void* out, int images, int height, int width, int rows,
                            int cols, cudaStream_t stream);
 
+// Rows of `vocab` logits in two levels of strides, in elements: row r starts at
+// (r / inner) * outer_stride + (r % inner) * row_stride.
+enum class LogitType { kFloat, kBFloat16, kHalf };
+struct LogitRows {
+  int64_t rows, inner, outer_stride, row_stride;
+  int vocab;
+  LogitType type;
+};
+
+// Log probabilities of `tokens` (may be null: no token is asked for) at a temperature, the entropy and the `k` largest
+// entries; outputs that are null or of k = 0 are left out.  `stats`, 2 floats a row, is for the backward.  A row whose
+// token is negative does not count; one whose token is past the vocabulary has the log probability NaN.
+constexpr int kMostTopTokens = 128;
+struct TokenLogProbsArgs {
+  const int64_t* tokens;
+  double temperature;
+  float* log_probs;
+  float* entropy;
+  float* stats;
+  int k;
+  float* top_log_probs;
+  int64_t* top_tokens;
+};
+cudaError_t launchTokenLogProbs(const void* logits, const LogitRows& x, const TokenLogProbsArgs& a, int sm_count,
+                                cudaStream_t stream);
+// `grad` has the strides of the logits and lies as they do relative to a 16-byte boundary.  The gradients of the two
+// outputs are one value a row, `stride` floats apart (0: one value for all); either may be null.
+struct TokenLogProbsGrads {
+  const int64_t* tokens;
+  double temperature;
+  const float* stats;
+  const float* entropy;
+  const float* g_log_probs;
+  int64_t g_stride;
+  const float* g_entropy;
+  int64_t h_stride;
+};
+cudaError_t launchTokenLogProbsBackward(const void* logits, const LogitRows& x, void* grad, const TokenLogProbsGrads& a,
+                                        cudaStream_t stream);
+
+// Divergence of the rows' softmax from a teacher's `k` log probabilities a row; a negative token is padding.  `rest`:
+// what they leave of the probability, if it is more than the rounding of fp32 log probabilities, is one more class.  `stats` (4 floats a row) and `merged` (k pairs of token and
+// probability a row) are for the backward; `merged` may be null.
+constexpr int kMostTeacherTokens = 256;
+constexpr int kMostRestVocab = 1 << 20;
+constexpr double kLeastRest = 1.0 / (1 << 20);
+struct DistillationArgs {
+  const int64_t* tokens;
+  const float* log_probs;
+  int k;
+  double temperature;
+  bool rest;
+};
+cudaError_t launchDistillation(const void* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float* stats,
+                               void* merged, int sm_count, cudaStream_t stream);
+// *mean = sum of `loss` / *count, *count = number of rows that count, at least 1.
+cudaError_t launchDistillationMean(const float* loss, const float* stats, int64_t rows, float* mean, float* count,
+                                   cudaStream_t stream);
+// The gradient, scaled by upstream[row * stride] / *count (count may be null); `grad` as above.
+cudaError_t launchDistillationBackward(const void* logits, const LogitRows& x, void* grad, const float* stats,
+                                       const void* merged, int k, double temperature, const float* upstream, int64_t stride,
+                                       const float* count, cudaStream_t stream);
+
 uint64_t localLaunchCountImpl();
 void noteLocalLaunch();
 

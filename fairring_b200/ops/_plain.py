@@ -13,15 +13,19 @@ from torch.nn.modules import module as _module
 FUSE_FROM = 1 << 22
 
 
-def plain_autograd() -> bool:
+def plain_calls() -> bool:
     """False inside what looks through torch's own ops but not through a native kernel: tracing and
     compilation, dispatch modes (``make_fx``, fake tensors, FLOP counting), functorch (``vmap``,
-    ``grad``, ``jvp``), forward-mode differentiation; and in inference mode."""
+    ``grad``, ``jvp``) and forward-mode differentiation."""
     if torch.compiler.is_compiling():  # asked first: Dynamo refuses some of the questions below
         return False
     return not (torch.jit.is_tracing() or torch._C._len_torch_dispatch_stack() > 0
-                or torch.is_inference_mode_enabled() or torch._C._are_functorch_transforms_active()
-                or forward_ad._current_level >= 0)
+                or torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0)
+
+
+def plain_autograd() -> bool:
+    """As :func:`plain_calls`, and not in inference mode either, which an autograd function is not made for."""
+    return plain_calls() and not torch.is_inference_mode_enabled()
 
 
 def ordinary(x) -> bool:
