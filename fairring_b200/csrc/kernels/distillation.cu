@@ -14,60 +14,105 @@ namespace {
 
 using namespace softmax_row;
 
-static_assert(kMostTeacherTokens <= kThreads, "a thread per listed token");
-
+// What the teacher says of one row, and the student of the tokens that it names.
 struct Teacher {
-  int token[kMostTeacherTokens];    // -1: padding
-  float given[kMostTeacherTokens];  // the teacher's value
-  float logit[kMostTeacherTokens];  // the student's
+  alignas(16) int token[kMostTeacherTokens];  // -1: padding or no token
+  float given[kMostTeacherTokens];            // the teacher's value
+  float logit[kMostTeacherTokens];            // the student's
   float q[kMostTeacherTokens];
   bool first[kMostTeacherTokens];  // no entry before it names the same token
   double log_total;                // what turns the values into log probabilities
   double mass;                     // sum of q
 };
 
-__device__ __forceinline__ float warpMax(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
-  return v;
-}
-template <typename V> __device__ __forceinline__ V warpSum(V v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
-  return v;
-}
-
-// Takes the listed tokens' logits out of the sweep: one bit per column of the slice, a vector's bits in one byte.
-struct RestHook {
-  const unsigned char* bits;
-  int shift;  // bit of the slice's column c0, so that a vector's bits start at a multiple of its length
-  template <typename T> __device__ __forceinline__ unsigned of(int pos) const {
-    return bits[pos >> 3] >> (pos & 7) & ((1u << Vec<T>::kElems) - 1u);
+// The columns that the sweep leaves out, for a second look at a row.
+struct LeaveListed {
+  const Teacher* te;
+  int k;
+  __device__ __forceinline__ bool operator()(int col) const {
+    for (int i = 0; i < k; ++i)
+      if (te->token[i] == col) return true;
+    return false;
   }
-  template <typename T> __device__ __forceinline__ void mask(uint4 (&now)[kBatch], int i, const Slice<T>& sl) {
-    constexpr int E = Vec<T>::kElems;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int v = i + u * kThreads;
-      if (v >= sl.v1) continue;
-      const unsigned listed = of<T>(sl.head + v * E - sl.c0 + shift);
-      if (listed == 0) continue;
-      float2 x[E / 2];
-      Vec<T>::get(now[u], x);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        if (listed >> (2 * e) & 1u) x[e].x = -INFINITY;
-        if (listed >> (2 * e + 1) & 1u) x[e].y = -INFINITY;
-      }
-      now[u] = Vec<T>::set(x);
-    }
-  }
-  template <typename V>
-  __device__ __forceinline__ void batch(int, const uint4 (&)[kBatch], const float (&)[kBatch], float, int, const V&) {}
 };
 
-// The teacher's probabilities, by one warp.
-template <bool kRest> __device__ __forceinline__ void teacherOf(Teacher& te, int k, float inv_t) {
+// Takes the listed tokens' logits out of the sweep: a bit for each column of the slice's vectors, so that the bits of what one
+// thread has of a batch are one word (16 bits of fp32 logits), and a word for the columns outside the vectors.
+template <typename T> struct Marks {
+  static constexpr int E = Vec<T>::kElems, kBits = kBatch * E;
+  // Whole batches, and at least one: a row without a vector is swept as a batch of none.
+  static __host__ __device__ __forceinline__ int words(int vecs) {
+    const int batches = (vecs + kBatch * kThreads - 1) / (kBatch * kThreads);
+    return (batches > 0 ? batches : 1) * kThreads * kBits / 32;
+  }
+  static __device__ __forceinline__ bool loose(const Slice<T>& sl, int col) { return col < sl.firstCol() || col >= sl.lastCol(); }
+  static __device__ __forceinline__ unsigned looseBit(const Slice<T>& sl, int col) {
+    return 1u << (col < sl.firstCol() ? col - sl.c0 : col - sl.lastCol() + sl.firstCol() - sl.c0);
+  }
+  static __device__ __forceinline__ unsigned place(const Slice<T>& sl, int col) {
+    const unsigned v = (unsigned)(col - sl.firstCol()) / E, e = (unsigned)(col - sl.firstCol()) % E;
+    return (v / (kBatch * kThreads) * kThreads + v % kThreads) * kBits + v / kThreads % kBatch * E + e;
+  }
+};
+// Whether the bit was set before.
+__device__ __forceinline__ bool setBit(unsigned* bits, unsigned at) {
+  return atomicOr(&bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u;
+}
+__device__ __forceinline__ void clearBit(unsigned* bits, unsigned at) { atomicAnd(&bits[at >> 5], ~(1u << (at & 31))); }
+
+struct RestHook {
+  const unsigned* bits;
+  // Those of what this thread has of batch b.
+  template <typename T> __device__ __forceinline__ unsigned listed(int b) const {
+    const int unit = b * kThreads + (int)threadIdx.x;
+    return Marks<T>::kBits == 32 ? bits[unit] : reinterpret_cast<const unsigned short*>(bits)[unit];
+  }
+  template <typename T> __device__ __forceinline__ float batch(uint4 (&now)[kBatch], bool, int i, const Slice<T>& sl) {
+    constexpr int E = Vec<T>::kElems;
+    const unsigned mine = listed<T>((i - sl.v0) / (kBatch * kThreads));
+    if (__any_sync(kAll, mine != 0)) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (!__any_sync(kAll, (mine >> (u * E) & ((1u << E) - 1u)) != 0)) continue;
+        float2 x[E / 2];
+        Vec<T>::get(now[u], x);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          if (mine >> (u * E + 2 * e) & 1u) x[e].x = -INFINITY;
+          if (mine >> (u * E + 2 * e + 1) & 1u) x[e].y = -INFINITY;
+        }
+        now[u] = Vec<T>::set(x);
+      }
+    }
+    return batchMax<T>(now);
+  }
+};
+
+// The entries of row r, by one warp; returns whether one is past the vocabulary.  Then the student's logits of those tokens.
+__device__ __forceinline__ bool loadTeacher(Teacher& te, const int64_t* tokens, const float* log_probs, int k, int64_t r,
+                                            int vocab) {
+  const int lane = threadIdx.x & 31;
+  bool outside = false;
+#pragma unroll 4
+  for (int i = lane; i < k; i += 32) {
+    const int64_t t = tokens[r * k + i];
+    te.given[i] = log_probs[r * k + i];
+    te.token[i] = t < 0 || t >= vocab ? -1 : (int)t;
+    outside |= t >= vocab;
+  }
+  if (lane < 4 && k + lane < kMostTeacherTokens) te.token[k + lane] = -2;
+  __syncwarp();
+  return __any_sync(kAll, outside);
+}
+template <typename T> __device__ __forceinline__ void loadLogits(Teacher& te, int k, const T* row) {
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < k; i += 32) te.logit[i] = te.token[i] >= 0 ? toFloat(row[te.token[i]]) : 0.f;
+  __syncwarp();
+}
+
+// The teacher's probabilities, and with `merged` the listed tokens, each once, with the sum of what its entries
+// have, by one warp.  `twice`: a token may be named more than once.
+template <bool kRest> __device__ __forceinline__ void teacherOf(Teacher& te, int k, float inv_t, bool twice, int2* merged) {
   const int lane = threadIdx.x & 31;
   if constexpr (kRest) {
     double mass = 0;
@@ -92,59 +137,143 @@ template <bool kRest> __device__ __forceinline__ void teacherOf(Teacher& te, int
     for (int i = lane; i < k; i += 32) te.q[i] /= total;
     if (lane == 0) te.mass = 1, te.log_total = (double)top * inv_t + log((double)total);
   }
+  __syncwarp();
+  if (!kRest && merged == nullptr) return;
+  if (!twice) {
+    for (int i = lane; i < k; i += 32) {
+      te.first[i] = te.token[i] >= 0;
+      if (merged != nullptr) merged[i] = make_int2(te.token[i], __float_as_int(te.q[i]));
+    }
+    __syncwarp();
+    return;
+  }
+  for (int i = lane; i < k; i += 32) {
+    const int t = te.token[i];
+    float q = 0.f;
+    int before = k;
+    for (int j = 0; j < k; j += 4) {  // four at a time; behind the last of them is no token
+      const int4 o = *reinterpret_cast<const int4*>(&te.token[j]);
+      if (o.x == t) q += te.q[j], before = min(before, j);
+      if (o.y == t) q += te.q[j + 1], before = min(before, j + 1);
+      if (o.z == t) q += te.q[j + 2], before = min(before, j + 2);
+      if (o.w == t) q += te.q[j + 3], before = min(before, j + 3);
+    }
+    const bool first = t >= 0 && before == i;
+    te.first[i] = first;
+    if (merged != nullptr) merged[i] = make_int2(first ? t : -1, __float_as_int(q));
+  }
+  __syncwarp();
 }
 
-// One row per cluster.  Kept for the backward: the maximum that its sweep takes differences from and the factor of
-// those exponentials, the same for the listed tokens; the last is -1 where the row does not count.  The listed
-// tokens with the probabilities of equal ones added up, each once, are written to `merged`.
+// Loss and what the backward needs, from the sums of the sweep, by one warp.  Kept: the maximum that the sweep takes
+// differences from and the factor of those exponentials, the same for the listed tokens; the last is -1 where the row does
+// not count.
+template <bool kRest>
+__device__ __forceinline__ void finishRow(const Teacher& te, int k, const Sums& acc, bool broken, float c, double inv_t, float* loss,
+                                          float4* stats) {
+  const int lane = threadIdx.x & 31;
+  // All probabilities' maximum and sum; the sweep's are those of the rest.
+  float m = acc.m, s = acc.s;
+  if constexpr (kRest) {
+    for (int i = lane; i < k; i += 32)
+      if (te.first[i]) m = fmaxf(m, te.logit[i]);
+    m = warpMax(m);
+    float sum = 0.f;
+    for (int i = lane; i < k; i += 32)
+      if (te.first[i]) sum += exp2Of((te.logit[i] - m) * c);
+    s = acc.s * exp2Of((acc.m - m) * c) + warpSum(sum);
+  }
+  // A divergence is a small difference of large logarithms: those are kept in 64 bits.
+  const double lse = (double)m * inv_t + log((double)s);
+  double sum = 0;
+  for (int i = lane; i < k; i += 32) {
+    const float q = te.q[i];
+    if (te.token[i] >= 0 && !(q == 0.f)) {
+      const double log_q = kRest ? (double)te.given[i] : (double)te.given[i] * inv_t - te.log_total;
+      sum += q * (log_q - ((double)te.logit[i] * inv_t - lse));
+    }
+  }
+  sum = warpSum(sum);
+  if (lane != 0) return;
+  const float nan = __int_as_float(0x7fffffff);  // NaN
+  float4 st = make_float4(m, 1.f / s, m, 1.f / s);
+  if constexpr (kRest) {
+    const double q_rest = 1.0 - te.mass < kLeastRest ? 0.0 : 1.0 - te.mass;  // NaN stays
+    if (!(q_rest == 0)) sum += q_rest * (log(q_rest) - ((double)acc.m * inv_t + log((double)acc.s) - lse));
+    const double all = te.mass + q_rest, p_rest = (double)(acc.s * exp2Of((acc.m - m) * c)) / s;
+    const bool some = !(acc.s == 0.f);
+    st = make_float4(some ? acc.m : 0.f, some ? (float)((all * p_rest - q_rest) / acc.s) : 0.f, m, (float)(all / s));
+  }
+  st.y *= exp2Of(-Exponent::excess(st.x, c));
+  st.w *= exp2Of(-Exponent::excess(st.z, c));
+  *stats = broken ? make_float4(nan, nan, nan, nan) : st;
+  *loss = broken ? nan : (float)sum;
+}
+
+// A row counts that has a listed token and, without the rest, one that the teacher gives some probability.
+template <bool kRest> struct Counts {
+  const int64_t* tokens;
+  const float* log_probs;
+  int k;
+  __device__ __forceinline__ bool entry(int64_t r, int i) const {
+    return tokens[r * k + i] >= 0 && (kRest || !(log_probs[r * k + i] == -INFINITY));
+  }
+  __device__ __forceinline__ bool operator()(int r) const {
+    bool some = entry(r, 0);
+    for (int i = 1; i < k && !some; ++i) some = entry(r, i);
+    return some;
+  }
+};
+
+__device__ __forceinline__ void skipRow(float* loss, float4* stats) {
+  *loss = 0.f;
+  *stats = make_float4(0.f, 0.f, 0.f, -1.f);
+}
+
+// Few rows: one per cluster.
 template <typename T, bool kRest>
 __global__ void __launch_bounds__(kThreads, 4)
-distillation_fwd_kernel(const T* __restrict__ logits, LogitRows x, const int64_t* __restrict__ tokens,
-                        const float* __restrict__ log_probs, int k, float c, double inv_t, float* __restrict__ loss,
-                        float4* __restrict__ stats, int2* __restrict__ merged) {
+distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRest> given, float c, double inv_t,
+                           float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged) {
   namespace cg = cooperative_groups;
   __shared__ Teacher te;
   __shared__ Sums scratch[kWarps], mine;
+  __shared__ unsigned loose;
   extern __shared__ __align__(16) unsigned bits[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.num_blocks(), rank = cluster.block_rank();
   const int64_t r = blockIdx.x / slices;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, k = given.k;
   const T* row = rowOf(x, logits, r);
   const Slice<T> sl(row, x.vocab, rank, slices);
-  bool counts = false, outside = false;
-  if (tid < k) {
-    const int64_t t = tokens[r * k + tid];
-    const float given = log_probs[r * k + tid];
-    outside = t >= x.vocab;
-    te.token[tid] = t < 0 || outside ? -1 : (int)t;
-    te.given[tid] = given;
-    counts = t >= 0 && (kRest || !(given == -INFINITY));
-    if (rank == 0) te.logit[tid] = t < 0 || outside ? 0.f : toFloat(row[t]);
-  }
   RestHook hook;
-  if constexpr (kRest) {
-    hook.bits = reinterpret_cast<const unsigned char*>(bits);
-    hook.shift = (Vec<T>::kElems - (sl.firstCol() - sl.c0) % Vec<T>::kElems) % Vec<T>::kElems;
-    for (int i = tid; i < (sl.c1 - sl.c0 + hook.shift + 31) / 32; i += kThreads) bits[i] = 0;
-  }
-  counts = __syncthreads_or(counts);
-  outside = __syncthreads_or(outside);
-  if (!counts) {
-    if (rank == 0 && tid == 0) {
-      loss[r] = 0.f;
-      stats[r] = make_float4(0.f, 0.f, 0.f, -1.f);
-    }
+  hook.bits = bits;
+  if (tid == 0) loose = 0;
+  if constexpr (kRest)
+    for (int i = tid; i < Marks<T>::words(sl.v1 - sl.v0); i += kThreads) bits[i] = 0;
+  bool some = false;
+  for (int i = tid; i < k; i += kThreads) some |= given.entry(r, i);
+  if (!__syncthreads_or(some)) {
+    if (rank == 0 && tid == 0) skipRow(loss + r, stats + r);
     return;
   }
   if constexpr (kRest) {
-    if (tid < k) {
-      const int t = te.token[tid], pos = t - sl.c0 + hook.shift;
-      if (t >= sl.c0 && t < sl.c1) atomicOr(&bits[pos >> 5], 1u << (pos & 31));
+    for (int i = tid; i < k; i += kThreads) {
+      const int64_t t = given.tokens[r * k + i];
+      if (t < sl.c0 || t >= sl.c1) continue;
+      if (Marks<T>::loose(sl, (int)t))
+        atomicOr(&loose, Marks<T>::looseBit(sl, (int)t));
+      else
+        setBit(bits, Marks<T>::place(sl, (int)t));
     }
     __syncthreads();
   }
-  if (rank == 0 && tid < 32) teacherOf<kRest>(te, k, (float)inv_t);
+  bool outside = false;
+  if (rank == 0 && tid < 32) {
+    outside = loadTeacher(te, given.tokens, given.log_probs, k, r, x.vocab);
+    loadLogits(te, k, row);
+    teacherOf<kRest>(te, k, (float)inv_t, true, merged != nullptr ? merged + r * k : nullptr);
+  }
   Sums acc;
   if constexpr (kRest) {
     acc = scan<T, false>(sl, c, hook);
@@ -154,68 +283,124 @@ distillation_fwd_kernel(const T* __restrict__ logits, LogitRows x, const int64_t
   }
   if (tid < 2 * Vec<T>::kElems) {
     const int col = sl.looseCol(tid);
-    bool listed = false;
-    if constexpr (kRest) {
-      const int pos = col - sl.c0 + hook.shift;
-      listed = col >= 0 && (bits[pos >> 5] >> (pos & 31) & 1u);
-    }
-    if (col >= 0 && !listed) acc.add<false>(toFloat(row[col]), c);
+    if (col >= 0 && !(loose >> tid & 1u)) acc.add<false>(toFloat(row[col]), c);
   }
   acc = blockSums<false>(acc, c, scratch);
   if (slices > 1) {
     acc = clusterSums<false>(acc, c, &mine);
     clusterDone();
-    if (rank != 0) return;
   }
-  if (tid < k) {
-    const int t = te.token[tid];
-    float q = 0.f;
-    bool first = t >= 0;
-    for (int j = 0; j < k; ++j)
-      if (te.token[j] == t) {
-        q += te.q[j];
-        first = first && j >= tid;
-      }
-    te.first[tid] = first;
-    if (merged != nullptr) merged[r * k + tid] = make_int2(first ? t : -1, __float_as_int(q));
+  if (rank != 0) return;
+  if (!acc.settle<false>(c)) {
+    if constexpr (kRest)
+      acc = blockAgain<T, false>(row, x.vocab, c, scratch, LeaveListed{&te, k});
+    else
+      acc = blockAgain<T, false>(row, x.vocab, c, scratch, LeaveNone());
   }
-  __syncthreads();
-  if (tid >= 32) return;
-  // All probabilities' maximum and sum; the sweep's are those of the rest.
-  float m = acc.m, s = acc.s;
-  if constexpr (kRest) {
-    for (int i = tid; i < k; i += 32)
-      if (te.first[i]) m = fmaxf(m, te.logit[i]);
-    m = warpMax(m);
-    float sum = 0.f;
-    for (int i = tid; i < k; i += 32)
-      if (te.first[i]) sum += exp2Of((te.logit[i] - m) * c);
-    s = acc.s * exp2Of((acc.m - m) * c) + warpSum(sum);
+  if (tid < 32) finishRow<kRest>(te, k, acc, outside, c, inv_t, loss + r, stats + r);
+}
+
+// Many rows: the blocks stay.  With the rest a finishing warp marks the listed tokens of its next row while the rows before
+// it are swept, and takes the marks away when it is done.
+constexpr int kFinishers = 64, kFinishWarps = kFinishers / 32;
+constexpr int kUnfinished = kFinishWarps;
+constexpr int kNameWords = 1024;
+struct DistillRows {
+  Ring ring;
+  HandOver<kUnfinished> hand;
+  Teacher teacher[kFinishWarps];
+  alignas(16) unsigned bits[1];  // words for each finishing warp: marks of a row's listed tokens
+};
+template <typename T> struct RestRowsHook : RestHook {
+  HandOver<kUnfinished>* hand;
+  const unsigned* all;
+  int words_a_row;
+  __device__ __forceinline__ void begin(int buffer, unsigned parity) {
+    hand->wait(&hand->ready[buffer], parity);
+    bits = all + buffer * words_a_row;
   }
-  // A divergence is a small difference of large logarithms: those are kept in 64 bits.
-  const double lse = (double)m * inv_t + log((double)s);
-  double sum = 0;
-  for (int i = tid; i < k; i += 32) {
-    const float q = te.q[i];
-    if (te.token[i] >= 0 && !(q == 0.f)) {
-      const double log_q = kRest ? (double)te.given[i] : (double)te.given[i] * inv_t - te.log_total;
-      sum += q * (log_q - ((double)te.logit[i] * inv_t - lse));
+  __device__ __forceinline__ void end() {}
+  __device__ __forceinline__ void arrived(uint4* place, int b) {
+    constexpr int E = Vec<T>::kElems;
+    for (unsigned mine = listed<T>(b); mine != 0; mine &= mine - 1) {
+      const int at = __ffs(mine) - 1;
+      fromFloat(reinterpret_cast<T*>(place + at / E * kThreads) + at % E, -INFINITY);
     }
   }
-  sum = warpSum(sum);
-  if (tid != 0) return;
-  const float nan = __int_as_float(0x7fffffff);
-  if constexpr (kRest) {
-    const double q_rest = 1.0 - te.mass < kLeastRest ? 0.0 : 1.0 - te.mass;  // NaN stays
-    if (!(q_rest == 0)) sum += q_rest * (log(q_rest) - ((double)acc.m * inv_t + log((double)acc.s) - lse));
-    const double all = te.mass + q_rest, p_rest = (double)(acc.s * exp2Of((acc.m - m) * c)) / s;
-    const bool some = !(acc.s == 0.f);
-    stats[r] = outside ? make_float4(nan, nan, nan, nan)
-                       : make_float4(some ? acc.m : 0.f, some ? (float)((all * p_rest - q_rest) / acc.s) : 0.f, m, (float)(all / s));
-  } else {
-    stats[r] = outside ? make_float4(nan, nan, nan, nan) : make_float4(m, 1.f / s, m, 1.f / s);
+  __device__ __forceinline__ float batch(uint4 (&now)[kBatch], bool, int, const Slice<T>&) { return batchMax<T>(now); }
+};
+template <typename T, bool kRest>
+__global__ void __launch_bounds__(kThreads + kFinishers, 3)
+distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRest> counts, float c, double inv_t,
+                         float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged, int words) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  DistillRows& shared = *reinterpret_cast<DistillRows*>(dynamic);
+  HandOver<kUnfinished>& hand = shared.hand;
+  if (threadIdx.x == 0) hand.init();
+  for (int i = threadIdx.x; i < words * kUnfinished; i += kThreads + kFinishers)
+    shared.bits[i] = 0;
+  __syncthreads();
+  if (threadIdx.x < kThreads) {
+    if constexpr (kRest) {
+      RestRowsHook<T> hook;
+      hook.hand = &hand;
+      hook.all = shared.bits;
+      hook.words_a_row = words;
+      sweepRows<T, false>(logits, x, counts, c, shared.ring, hand, hook);
+    } else {
+      NoHook none;
+      sweepRows<T, false>(logits, x, counts, c, shared.ring, hand, none);
+    }
+    return;
   }
-  loss[r] = outside ? nan : (float)sum;
+  const int which = (int)(threadIdx.x - kThreads) / 32, lane = threadIdx.x & 31, k = counts.k;
+  Teacher& te = shared.teacher[which];
+  const auto finish = [&](int64_t r, int buffer, unsigned parity) {
+    const T* row = rowOf(x, logits, r);
+    const Slice<T> sl(row, x.vocab, 0, 1);
+    const bool outside = loadTeacher(te, counts.tokens, counts.log_probs, k, r, x.vocab);
+    unsigned left_out = 0;
+    unsigned* bits = shared.bits + buffer * words;
+    bool twice = false;
+    if constexpr (kRest) {
+      for (int i = lane; i < k; i += 32) {
+        const int t = te.token[i];
+        if (t < 0) continue;
+        if (Marks<T>::loose(sl, t))
+          left_out |= Marks<T>::looseBit(sl, t), twice = true;  // perhaps: there are few
+        else
+          twice |= setBit(bits, Marks<T>::place(sl, t));
+      }
+      left_out = __reduce_or_sync(kAll, left_out);
+      if (lane == 0) barrierArrive(&hand.ready[buffer]);
+    } else {  // a token's bit is that of its number's end: two that differ may share it, which costs time alone
+      for (int i = lane; i < k; i += 32)
+        if (te.token[i] >= 0) twice |= setBit(bits, te.token[i] % (32 * kNameWords));
+      __syncwarp();
+      for (int i = lane; i < k; i += 32)
+        if (te.token[i] >= 0) clearBit(bits, te.token[i] % (32 * kNameWords));
+    }
+    teacherOf<kRest>(te, k, (float)inv_t, __any_sync(kAll, twice), merged != nullptr ? merged + r * k : nullptr);
+    hand.wait(&hand.full[buffer], parity);
+    loadLogits(te, k, row);  // swept not long ago: from L2
+    Sums acc = hand.template take<T, false>(buffer, sl, c, left_out);
+    if constexpr (kRest)
+      for (int i = lane; i < k; i += 32)
+        if (te.token[i] >= 0 && !Marks<T>::loose(sl, te.token[i])) clearBit(bits, Marks<T>::place(sl, te.token[i]));
+    __syncwarp();
+    if (lane == 0) barrierArrive(&hand.empty[buffer]);
+    if (!acc.settle<false>(c)) {
+      if constexpr (kRest)
+        acc = warpAgain<T, false>(row, x.vocab, c, LeaveListed{&te, k});
+      else
+        acc = warpAgain<T, false>(row, x.vocab, c, LeaveNone());
+    }
+    finishRow<kRest>(te, k, acc, outside || hand.gaveUp(), c, inv_t, loss + r, stats + r);
+    __syncwarp();
+  };
+  finishRows<kUnfinished>(counts, x.rows, which, kFinishWarps, finish, [&](int64_t r) {
+    if (which == 0) skipRow(loss + r, stats + r);
+  });
 }
 
 __global__ void __launch_bounds__(1024)
@@ -273,8 +458,9 @@ distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, cons
     }
     const float up = upstream[r * stride] * inv_t, g = count != nullptr ? up / *count : up;
     const float f = st.y * g;
+    const Exponent exponent(st.x, c);
     auto of = [&](float2 v) {
-      const float2 d = mul2(add2(v, make_float2(-st.x, -st.x)), make_float2(c, c));
+      const float2 d = exponent(v);
       return mul2(make_float2(exp2Of(d.x), exp2Of(d.y)), make_float2(f, f));
     };
 #pragma unroll
@@ -297,30 +483,42 @@ distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, cons
     }
     if (counts) {
       __syncthreads();  // the block's stores before those of the listed tokens
-      if (mine.x >= 0) fromFloat(out + mine.x, fmaf(exp2Of((logit - st.z) * c), st.w, -__int_as_float(mine.y)) * g);
+      if (mine.x >= 0) fromFloat(out + mine.x, fmaf(exp2Of(Exponent(st.z, c)(make_float2(logit, 0.f)).x), st.w, -__int_as_float(mine.y)) * g);
     }
   }
+}
+
+template <typename T, bool kRest>
+cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float4* stats, int2* merged,
+                      int sm_count, cudaStream_t stream) {
+  const float c = (float)(1.4426950408889634 / a.temperature);
+  const double inv_t = 1.0 / a.temperature;
+  const Counts<kRest> counts{a.tokens, a.log_probs, a.k};
+  const int words = kRest ? Marks<T>::words(x.vocab / Vec<T>::kElems) : kNameWords;
+  const size_t stay = sizeof(DistillRows) + kUnfinished * (size_t)words * 4;
+  // Two blocks of the form that stays have to fit on a multiprocessor, with up to 70,000 tokens three do.
+  if (manyRows(x.rows, sm_count) && stay <= 112 * 1024)
+    return launchResident(distillation_rows_kernel<T, kRest>, x.rows, kThreads + kFinishers, stay <= 75 * 1024 ? 3 : 2, stay, sm_count,
+                          stream, logits, x, counts, c, inv_t, loss, stats, merged, words);
+  const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
+  const size_t shared = kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) * 4 : 0;
+  if (shared > 32 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(distillation_slices_kernel<T, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)shared);
+    if (e != cudaSuccess) return e;
+  }
+  return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, shared, stream, logits, x, counts, c, inv_t, loss,
+                      stats, merged);
 }
 
 template <typename T>
 cudaError_t forwardOf(const void* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float* stats,
                       void* merged, int sm_count, cudaStream_t stream) {
-  const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
-  const float c = (float)(1.4426950408889634 / a.temperature);
-  auto run = [&](auto kernel, size_t shared) {
-    return launchSlices(kernel, x.rows, slices, shared, stream, static_cast<const T*>(logits), x, a.tokens, a.log_probs, a.k,
-                        c, 1.0 / a.temperature, loss, reinterpret_cast<float4*>(stats), static_cast<int2*>(merged));
-  };
-  if (!a.rest) return run(distillation_fwd_kernel<T, false>, 0);
-  // The widest slice in whole vectors, its row's head and tail, and the shift of its first bit.
-  constexpr int E = Vec<T>::kElems;
-  const size_t shared = ((((int64_t)x.vocab / E + slices - 1) / slices * E + 3 * E) / 32 + 1) * 4;
-  if (shared > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(distillation_fwd_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)shared);
-    if (e != cudaSuccess) return e;
-  }
-  return run(distillation_fwd_kernel<T, true>, shared);
+  const T* data = static_cast<const T*>(logits);
+  float4* st = reinterpret_cast<float4*>(stats);
+  int2* pairs = static_cast<int2*>(merged);
+  return a.rest ? forwardOf<T, true>(data, x, a, loss, st, pairs, sm_count, stream)
+                : forwardOf<T, false>(data, x, a, loss, st, pairs, sm_count, stream);
 }
 
 template <typename T>

@@ -6,9 +6,11 @@
 // block takes a row or, where there are few rows, the blocks of a cluster take a slice of it each and the first
 // one merges what they found, in the order of the slices.
 //
-// exp() is 2^((x - m) * c) with c = log2(e) / T.  The difference is taken before the product: m * c of a row
-// that is masked with the type's lowest value throughout would be minus infinity.  The exponential's own error
-// is 2^-22 of a probability, the two roundings before it 2^-23 of the exponent.
+// exp() is 2^((x - m) * c) with c = log2(e) / T, as one fused multiply-add of x, c and the rounded m * c; what that
+// rounding changes all exponentials by is put right at the row's end.  The exponential's own error is 2^-22 of a
+// probability.  That form needs |m * c| < 2^20.  A thread's m starts at -2^20 / c, below which nothing is seen of a row unless
+// all of it is there; such rows (masked with the type's lowest value throughout, or with minus infinity), those above and those with
+// a NaN come out of the sweep with a sum that is no positive number and are looked at again, slowly.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -31,6 +33,7 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr float kLn2 = 0.693147180559945309f;
 // exp2() of it is zero, and times it still is: in place of minus infinity where the exponent is a factor.
 constexpr float kLowExponent = -256.f;
+constexpr float kPlainRange = 1048576.f;
 
 template <typename T> struct Vec;
 template <> struct Vec<float> {
@@ -90,6 +93,13 @@ template <> struct Vec<__half> {
   }
 };
 
+// The largest of a batch, compared in the type that the values have.
+template <typename T> __device__ __forceinline__ float batchMax(const uint4 (&now)[kBatch]) {
+  float top = Vec<T>::max(now[0]);
+  for (int u = 1; u < kBatch; ++u) top = fmaxf(top, Vec<T>::max(now[u]));
+  return top;
+}
+
 __device__ __forceinline__ float toFloat(float v) { return v; }
 __device__ __forceinline__ float toFloat(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float toFloat(__half v) { return __half2float(v); }
@@ -130,6 +140,18 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(packed(a)), "l"(packed(b)), "l"(packed(c)));
   return unpacked(r);
 }
+
+// Threads that finish a row together: all of a block, or some warps of it under a barrier of their own.
+struct BlockGroup {
+  static constexpr int kSize = kThreads;
+  static __device__ __forceinline__ int rank() { return threadIdx.x; }
+  static __device__ __forceinline__ void sync() { __syncthreads(); }
+};
+template <int kFirst, int kCount, int kBarrier> struct PartGroup {
+  static constexpr int kSize = kCount;
+  static __device__ __forceinline__ int rank() { return (int)threadIdx.x - kFirst; }
+  static __device__ __forceinline__ void sync() { asm volatile("bar.sync %0, %1;" ::"n"(kBarrier), "n"(kCount) : "memory"); }
+};
 
 template <typename T> __device__ __forceinline__ T* rowOf(const LogitRows& x, T* data, int64_t r) {
   const int64_t outer = x.inner == x.rows ? 0 : r / x.inner;
@@ -172,52 +194,107 @@ template <typename T> struct Slice {
   }
 };
 
+// m * c, rounded wherever it stands: never a part of a fused multiply-add.
+__device__ __forceinline__ float scaled(float m, float c) { return __fmul_rn(m, c); }
+
+// The sums of a row or a part of it, while it is swept relative to the rounded m * c, in the end to m itself.
 struct Sums {
-  float m = -INFINITY, s = 0.f, a = 0.f;
-  // What differences are taken from: never -inf, whose difference from itself is NaN.
-  static __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
-  // The sums relative to `ref`, which is at least m.
-  template <bool kEntropy> __device__ __forceinline__ void rescale(float ref, float c) {
-    const float d = (m - ref) * c, f = exp2Of(d);
+  float m, s, a;
+  // Makes them 2^d times what they are, which raises every exponent by d.
+  template <bool kEntropy> __device__ __forceinline__ void shift(float d) {
+    const float f = exp2Of(d);
     if (kEntropy) a = f * fmaf(fmaxf(d, kLowExponent), s, a);
     s *= f;
   }
+  static __device__ __forceinline__ Sums none(float c) { return {-kPlainRange / c, 0.f, 0.f}; }
   template <bool kEntropy> __device__ __forceinline__ void merge(Sums o, float c) {
-    const float top = fmaxf(m, o.m), ref = reference(top);
-    rescale<kEntropy>(ref, c);
-    o.template rescale<kEntropy>(ref, c);
+    const float top = fmaxf(m, o.m), at = scaled(top, c);
+    shift<kEntropy>(scaled(m, c) - at);
+    o.template shift<kEntropy>(scaled(o.m, c) - at);
+    m = top;
     s += o.s;
     if (kEntropy) a += o.a;
-    m = top;
   }
   template <bool kEntropy> __device__ __forceinline__ void add(float v, float c) {
-    Sums o;
-    o.m = v;
-    o.s = v == -INFINITY ? 0.f : 1.f;
-    if (v != v) o.m = -INFINITY, o.s = v;
-    merge<kEntropy>(o, c);
+    const float top = fmaxf(m, v), at = scaled(top, c), d = fmaf(v, c, -at), e = exp2Of(d);
+    shift<kEntropy>(scaled(m, c) - at);
+    m = top;
+    s += e;
+    if (kEntropy) a = fmaf(e, fmaxf(d, kLowExponent), a);
   }
-  template <bool kEntropy> __device__ __forceinline__ Sums fromLane(int lane_mask) const {
-    Sums o;
-    o.m = __shfl_xor_sync(kAll, m, lane_mask);
-    o.s = __shfl_xor_sync(kAll, s, lane_mask);
-    if (kEntropy) o.a = __shfl_xor_sync(kAll, a, lane_mask);
-    return o;
+  // Relative to m; false for a row that has to be looked at again.
+  template <bool kEntropy> __device__ __forceinline__ bool settle(float c) {
+    shift<kEntropy>(-fmaf(m, c, -scaled(m, c)));
+    return scaled(m, c) < kPlainRange && s > 0.f && s < INFINITY;
   }
 };
 
-// What a kernel may do with a batch of vectors before they are summed: nothing.
+// A thread's share of a row, from the first of its vectors on.
+struct ThreadSums {
+  float m, at;  // at = m * c
+  float2 s, a;
+  __device__ __forceinline__ explicit ThreadSums(float c) : m(-kPlainRange / c), at(scaled(m, c)), s{0.f, 0.f}, a{0.f, 0.f} {}
+  // Adds the first n vectors of a batch whose largest value is `top`; all lanes of a warp have the same n.
+  template <typename T, bool kEntropy, bool kWhole>
+  __device__ __forceinline__ void add(const uint4 (&now)[kBatch], float top, int n, float c) {
+    constexpr int E = Vec<T>::kElems;
+    m = fmaxf(m, top);
+    const float before = at;
+    at = scaled(m, c);
+    const float d = before - at, f = exp2Of(d);
+    if (kEntropy) a = mul2(fma2(make_float2(fmaxf(d, kLowExponent), fmaxf(d, kLowExponent)), s, a), make_float2(f, f));
+    s = mul2(s, make_float2(f, f));
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (!kWhole && u >= n) break;
+      float2 v[E / 2];
+      Vec<T>::get(now[u], v);
+#pragma unroll
+      for (int k = 0; k < E / 2; ++k) {
+        const float2 d = fma2(v[k], make_float2(c, c), make_float2(-at, -at));
+        const float2 e = make_float2(exp2Of(d.x), exp2Of(d.y));
+        s = add2(s, e);
+        if (kEntropy) a = fma2(e, make_float2(fmaxf(d.x, kLowExponent), fmaxf(d.y, kLowExponent)), a);
+      }
+    }
+  }
+  __device__ __forceinline__ Sums sums() const { return {m, s.x + s.y, a.x + a.y}; }
+};
+
+// (x - m) * c of two values, for the backward kernels, too large by excess(m, c).
+struct Exponent {
+  float scale, minus, shift;
+  static __device__ __forceinline__ float excess(float m, float c) {
+    const float at = __fmul_rn(m, c);
+    return fabsf(at) < kPlainRange ? fmaf(m, c, -at) : 0.f;
+  }
+  __device__ __forceinline__ Exponent(float m, float c) {
+    const float at = __fmul_rn(m, c);
+    const bool plain = fabsf(at) < kPlainRange;  // else the difference is taken first, and its product is exact enough
+    minus = plain ? 0.f : -m;
+    scale = c;
+    shift = plain ? -at : 0.f;
+  }
+  __device__ __forceinline__ float2 operator()(float2 v) const {
+    return fma2(add2(v, make_float2(minus, minus)), make_float2(scale, scale), make_float2(shift, shift));
+  }
+};
+
+// What a kernel does with a batch, that from vector i on, before it is summed; returns its largest value.
 struct NoHook {
-  template <typename V> __device__ __forceinline__ void mask(uint4 (&)[kBatch], int, const V&) {}
-  template <typename V>
-  __device__ __forceinline__ void batch(int, const uint4 (&)[kBatch], const float (&)[kBatch], float, int, const V&) {}
+  __device__ __forceinline__ void begin(int, unsigned) {}
+  __device__ __forceinline__ void end() {}
+  __device__ __forceinline__ void arrived(uint4*, int) {}
+  template <typename T> __device__ __forceinline__ float batch(uint4 (&now)[kBatch], bool, int, const Slice<T>&) {
+    return batchMax<T>(now);
+  }
 };
 
-// This thread's sums over its share of the slice.  All threads of a block go through the same number of batches.
-// The next batch is on its way while this one is used.
+// This thread's share of the slice.  All threads of a block go through the same number of batches.  The next batch is on its
+// way while this one is used.
 template <typename T, bool kEntropy, class Hook>
 __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
-  constexpr int E = Vec<T>::kElems, U = kBatch;
+  constexpr int U = kBatch;
   constexpr uint32_t w = Vec<T>::kMinusInf;
   const uint4* vecs = reinterpret_cast<const uint4*>(sl.row + sl.head);
   uint4 raw[U];
@@ -226,7 +303,7 @@ __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
     for (int u = 0; u < U; ++u)
       raw[u] = i + u * kThreads < sl.v1 ? __ldg(vecs + i + u * kThreads) : make_uint4(w, w, w, w);
   };
-  Sums acc;
+  ThreadSums acc(c);
   const int batches = (sl.v1 - sl.v0 + U * kThreads - 1) / (U * kThreads);
   int i = sl.v0 + (int)threadIdx.x;
   fetch(i);
@@ -235,41 +312,54 @@ __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = raw[u];
     fetch(i + U * kThreads);
-    hook.mask(now, i, sl);
-    float vmax[U], top = acc.m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      vmax[u] = Vec<T>::max(now[u]);
-      top = fmaxf(top, vmax[u]);
-    }
-    hook.batch(b, now, vmax, top, i, sl);
-    const float ref = Sums::reference(top);
-    const float2 minus = make_float2(-ref, -ref), cc = make_float2(c, c);
-    float2 s2 = make_float2(0.f, 0.f), a2 = s2;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float2 v[E / 2];
-      Vec<T>::get(now[u], v);
-#pragma unroll
-      for (int k = 0; k < E / 2; ++k) {
-        const float2 d = mul2(add2(v[k], minus), cc);
-        const float2 e = make_float2(exp2Of(d.x), exp2Of(d.y));
-        s2 = add2(s2, e);
-        if (kEntropy) a2 = fma2(e, make_float2(fmaxf(d.x, kLowExponent), fmaxf(d.y, kLowExponent)), a2);
-      }
-    }
-    acc.rescale<kEntropy>(ref, c);
-    acc.s += s2.x + s2.y;
-    if (kEntropy) acc.a += a2.x + a2.y;
-    acc.m = top;
+    acc.add<T, kEntropy, false>(now, hook.batch(now, b == 0, i, sl), (sl.v1 - (i & ~31) + kThreads - 1) / kThreads, c);
+  }
+  return acc.sums();
+}
+
+// Two sweeps over a row for what the fast one cannot do, by `size` threads: this one's share of it, relative to m.
+template <typename T, bool kEntropy, class Leave>
+__device__ __noinline__ Sums lookAgain(const T* row, int vocab, int rank, int size, float c, float top, Leave leave) {
+  const float ref = top == -INFINITY ? 0.f : top;
+  Sums acc = {top, 0.f, 0.f};
+  for (int col = rank; col < vocab; col += size) {
+    if (leave(col)) continue;
+    const float d = (toFloat(row[col]) - ref) * c, e = exp2Of(d);
+    acc.s += e;
+    if (kEntropy) acc.a = fmaf(e, fmaxf(d, kLowExponent), acc.a);
   }
   return acc;
+}
+template <typename T, class Leave>
+__device__ __noinline__ float largestOf(const T* row, int vocab, int rank, int size, Leave leave) {
+  float top = -INFINITY;
+  for (int col = rank; col < vocab; col += size)
+    if (!leave(col)) top = fmaxf(top, toFloat(row[col]));
+  return top;
+}
+
+__device__ __forceinline__ float warpMax(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
+  return v;
+}
+template <typename V> __device__ __forceinline__ V warpSum(V v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// A warp's sums from its lanes', in every lane.
+template <bool kEntropy> __device__ __forceinline__ Sums warpSums(Sums acc, float c) {
+  const float m = warpMax(acc.m);
+  acc.shift<kEntropy>(scaled(acc.m, c) - scaled(m, c));
+  return {m, warpSum(acc.s), kEntropy ? warpSum(acc.a) : 0.f};
 }
 
 // The block's sums from its threads', in every thread.  `scratch`: kWarps of them in shared memory.
 template <bool kEntropy> __device__ __forceinline__ Sums blockSums(Sums acc, float c, Sums* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) acc.merge<kEntropy>(acc.fromLane<kEntropy>(o), c);
+  acc = warpSums<kEntropy>(acc, c);
+  __syncthreads();
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = acc;
   __syncthreads();
   acc = scratch[0];
@@ -277,6 +367,37 @@ template <bool kEntropy> __device__ __forceinline__ Sums blockSums(Sums acc, flo
   for (int i = 1; i < kWarps; ++i) acc.merge<kEntropy>(scratch[i], c);
   return acc;
 }
+
+// A row's sums, relative to m, by a whole block or a whole warp, where the sweep's did not settle.
+template <typename T, bool kEntropy, class Leave>
+__device__ __noinline__ Sums blockAgain(const T* row, int vocab, float c, Sums* scratch, Leave leave) {
+  float top = warpMax(largestOf(row, vocab, (int)threadIdx.x, kThreads, leave));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5].m = top;
+  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) top = fmaxf(top, scratch[i].m);
+  Sums acc = lookAgain<T, kEntropy>(row, vocab, (int)threadIdx.x, kThreads, c, top, leave);
+  acc.s = warpSum(acc.s);
+  acc.a = warpSum(acc.a);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = acc;
+  __syncthreads();
+  acc.s = acc.a = 0.f;
+  for (int i = 0; i < kWarps; ++i) acc.s += scratch[i].s, acc.a += scratch[i].a;
+  return acc;
+}
+template <typename T, bool kEntropy, class Leave>
+__device__ __noinline__ Sums warpAgain(const T* row, int vocab, float c, Leave leave) {
+  const int lane = threadIdx.x & 31;
+  const float top = warpMax(largestOf(row, vocab, lane, 32, leave));
+  Sums acc = lookAgain<T, kEntropy>(row, vocab, lane, 32, c, top, leave);
+  acc.s = warpSum(acc.s);
+  acc.a = warpSum(acc.a);
+  return acc;
+}
+struct LeaveNone {
+  __device__ __forceinline__ bool operator()(int) const { return false; }
+};
 
 // The row's sums from those of the slices' blocks, in the threads of block 0.  Every block of the cluster calls
 // it, and none leaves before clusterDone().
@@ -318,6 +439,219 @@ cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, si
   noteLocalLaunch();
   return e;
 }
+
+// ---- many rows -----------------------------------------------------------------
+// With a block per row the memory idles while a block starts and while it finishes its row, three to four
+// microseconds of the ten that the row itself takes (8192 x 51200 bf16: 144 us for the log probabilities, 4.6 to 5.8 TB/s).
+// So where there are many rows the blocks stay and take row after row in three roles:
+//  - eight warps sweep: every thread copies its own vectors to shared memory, kDepth - 1 batches ahead and
+//    across the ends of rows, and waits for its own copies alone;
+//  - they hand each row's sums over and go on without waiting;
+//  - the other warps finish rows: what needs no sums they do while the row is swept.
+constexpr int kManyRows = 4;  // for each multiprocessor
+constexpr int kDepth = 3;
+constexpr int kSpins = 1 << 20;  // tries, each of which the hardware lets sleep; then the wait is given up
+
+__device__ __forceinline__ uint32_t sharedAddress(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void barrierInit(uint64_t* bar, int arrivals) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sharedAddress(bar)), "r"(arrivals) : "memory");
+}
+__device__ __forceinline__ void barrierArrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sharedAddress(bar)) : "memory");
+}
+__device__ __forceinline__ bool barrierWait(uint64_t* bar, unsigned parity) {
+  for (int i = 0; i < kSpins; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(sharedAddress(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+__device__ __forceinline__ void copyAhead(uint4* to, const uint4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sharedAddress(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void waitCopies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+
+// The rows of this block that count, in order, as every warp finds them for itself: a lane looks at one of the next 32.
+template <class Counts> struct RowWalk {
+  const Counts& counts;
+  const unsigned rows;
+  unsigned base;      // the row of lane 0
+  unsigned mask = 0;  // of those not yet taken
+  int row = -1;       // the current one; -1: none left
+  __device__ __forceinline__ RowWalk(const Counts& counts_, int64_t rows_)
+      : counts(counts_), rows((unsigned)rows_), base(blockIdx.x - 32 * gridDim.x) {}
+  template <class Skip> __device__ __forceinline__ void next(Skip&& skip) {
+    while (mask == 0) {
+      base += 32 * gridDim.x;
+      if (base >= rows) {
+        base -= 32 * gridDim.x;
+        row = -1;
+        return;
+      }
+      const unsigned mine = base + (threadIdx.x & 31) * gridDim.x;
+      const bool some = mine < rows, yes = some && counts((int)mine);
+      if (some && !yes) skip((int)mine);
+      mask = __ballot_sync(kAll, yes);
+    }
+    row = (int)(base + (__ffs(mask) - 1) * gridDim.x);
+    mask &= mask - 1;
+  }
+  __device__ __forceinline__ void next() {
+    next([](int) {});
+  }
+};
+
+// What the sweeping warps hand over, for as many rows as may be unfinished at once.
+template <int kRows> struct HandOver {
+  // The row's listed tokens are marked; its sums are there; the buffer is free for another row.
+  uint64_t ready[kRows], full[kRows], empty[kRows];
+  Sums sums[kRows][kWarps];
+  int failed;
+  // By one thread, before a barrier of the block.
+  __device__ __forceinline__ void init() {
+    for (int i = 0; i < kRows; ++i) {
+      barrierInit(&ready[i], 1);
+      barrierInit(&full[i], kWarps);
+      barrierInit(&empty[i], 1);
+    }
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  // All lanes of a warp.  Once a wait was given up nobody waits any more, and the block's rows become NaN.
+  __device__ __forceinline__ void wait(uint64_t* bar, unsigned parity) {
+    if (!gaveUp() && !barrierWait(bar, parity)) *static_cast<volatile int*>(&failed) = 1;
+    __syncwarp();
+  }
+  // The row's sums in every lane of a warp; the columns outside the vectors are added here.
+  // `left_out`: a bit for each of those that is not to be.
+  template <typename T, bool kEntropy>
+  __device__ __forceinline__ Sums take(int buffer, const Slice<T>& sl, float c, unsigned left_out) const {
+    const int lane = threadIdx.x & 31;
+    Sums acc = lane < kWarps ? sums[buffer][lane] : Sums::none(c);
+    const int col = lane < 2 * Vec<T>::kElems && !(left_out >> lane & 1u) ? sl.looseCol(lane) : -1;
+    if (col >= 0) acc.add<kEntropy>(toFloat(sl.row[col]), c);
+    return warpSums<kEntropy>(acc, c);
+  }
+  __device__ __forceinline__ bool gaveUp() const { return *static_cast<const volatile int*>(&failed) != 0; }
+};
+
+using Ring = uint4[kDepth][kBatch][kThreads];
+
+// The sweeping warps' part, threads 0 to kThreads - 1.  The hook sees a thread's part of batch b of a row in shared memory
+// before it is read.
+template <typename T, bool kEntropy, int kRows, class Hook, class Counts>
+__device__ __forceinline__ void sweepRows(const T* logits, const LogitRows& x, const Counts& counts, float c, Ring& ring,
+                                          HandOver<kRows>& out, Hook& hook) {
+  constexpr int U = kBatch;
+  constexpr uint32_t w = Vec<T>::kMinusInf;
+  const int tid = threadIdx.x;
+  RowWalk<Counts> ahead(counts, x.rows), at(counts, x.rows);  // the row that is copied and the one that is summed
+  const uint4* from = nullptr;  // of the row that is copied: this thread's next vector,
+  int whole = 0, left = 0;      // the batches that all threads have, and the vectors from this thread's on behind those; < 0: no row
+  auto open = [&] {
+    ahead.next();
+    left = -kThreads;
+    if (ahead.row < 0) return;
+    const T* row = rowOf(x, logits, ahead.row);
+    const RowParts<T> parts(row, x.vocab);
+    from = reinterpret_cast<const uint4*>(row + parts.head) + tid;
+    whole = parts.nvec / (U * kThreads);
+    left = parts.nvec - whole * (U * kThreads);
+  };
+  auto issue = [&](int slot) {
+    uint4* to = &ring[slot][0][tid];
+    if (__any_sync(kAll, whole > 0)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) copyAhead(to + u * kThreads, from + u * kThreads);
+      from += U * kThreads;
+      if (--whole == 0 && left == 0) open();
+    } else if (left >= 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (tid + u * kThreads < left) copyAhead(to + u * kThreads, from + u * kThreads);
+      open();
+    }
+    commitCopies();
+  };
+  open();
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d) issue(d);
+  int slot = 0, buffer = 0;
+  unsigned parity = 0;
+  uint4 now[U];
+  auto take = [&](int b) {  // the row's batch b, whose turn it is; the place of the one before it, whose values have been used, is filled again
+    waitCopies<kDepth - 2>();
+    uint4* place = &ring[slot][0][tid];
+    hook.arrived(place, b);
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = place[u * kThreads];
+    issue(slot == 0 ? kDepth - 1 : slot - 1);
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
+  };
+  for (at.next(); at.row >= 0; at.next()) {
+    const Slice<T> sl(rowOf(x, logits, at.row), x.vocab, 0, 1);
+    out.wait(&out.empty[buffer], parity ^ 1);
+    hook.begin(buffer, parity);
+    ThreadSums mine(c);
+    const int batches = sl.v1 / (U * kThreads), rest = sl.v1 - batches * (U * kThreads);
+    for (int b = 0; b < batches; ++b) {
+      take(b);
+      mine.add<T, kEntropy, true>(now, hook.batch(now, b == 0, tid + b * (U * kThreads), sl), U, c);
+    }
+    if (rest > 0 || batches == 0) {
+      take(batches);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (tid + u * kThreads >= rest) now[u] = make_uint4(w, w, w, w);
+      mine.add<T, kEntropy, false>(now, hook.batch(now, batches == 0, tid + batches * (U * kThreads), sl),
+                                   (rest - (tid & ~31) + kThreads - 1) / kThreads, c);
+    }
+    hook.end();
+    const Sums acc = warpSums<kEntropy>(mine.sums(), c);
+    if ((tid & 31) == 0) {
+      out.sums[buffer][tid >> 5] = acc;
+      barrierArrive(&out.full[buffer]);
+    }
+    if (++buffer == kRows) buffer = 0, parity ^= 1;
+  }
+  waitCopies<0>();
+}
+
+// A finishing warp's or group's part: finish(row, buffer, parity) for those of the rows that count whose number is `which`
+// modulo `each`, skip(row) by single lanes for those that do not.
+template <int kRows, class Counts, class Finish, class Skip>
+__device__ __forceinline__ void finishRows(const Counts& counts, int64_t rows, int which, int each, Finish&& finish, Skip&& skip) {
+  RowWalk<Counts> at(counts, rows);
+  int buffer = 0, turn = 0;
+  unsigned parity = 0;
+  for (at.next(skip); at.row >= 0; at.next(skip)) {
+    if (turn == which) finish(at.row, buffer, parity);
+    if (++turn == each) turn = 0;
+    if (++buffer == kRows) buffer = 0, parity ^= 1;
+  }
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launchResident(void (*kernel)(Params...), int64_t rows, int threads, int blocks_per_sm, size_t shared,
+                           int sm_count, cudaStream_t stream, Args... args) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+  if (e != cudaSuccess) return e;
+  // Those that stay, or one for six rows: blocks do not get equal shares of the memory's bandwidth, and the hardware
+  // hands out the later ones to whoever is done.
+  const int64_t stay = (int64_t)blocks_per_sm * sm_count, blocks = rows / 6 > stay ? rows / 6 : stay;
+  kernel<<<(unsigned)(rows < blocks ? rows : blocks), threads, shared, stream>>>(Params(args)...);
+  noteLocalLaunch();
+  return cudaGetLastError();
+}
+
+// Whether rows are many enough for that: several for each of the blocks that stay.
+inline bool manyRows(int64_t rows, int sm_count) { return rows >= kManyRows * (int64_t)sm_count; }
 
 }  // namespace softmax_row
 }  // namespace fairring

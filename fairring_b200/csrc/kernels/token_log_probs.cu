@@ -3,6 +3,7 @@
 //
 // With z = x / T, m and S of softmax_row.cuh:  log p_v = (z_v - max z) - log S,  H = log S - A ln 2 / S, a sum of two
 // terms that are not negative.  Backward:  dx_v = 1/T [ g (1[v = t] - p_v) - h p_v (log p_v + H) ].
+#include <cfloat>
 #include <cmath>
 
 #include "softmax_row.cuh"
@@ -13,8 +14,10 @@ namespace {
 using namespace softmax_row;
 
 constexpr int kMostTop = kMostTopTokens;
-constexpr int kKeptVecs = 1024;  // vectors that may hold one of the largest
-constexpr int kList = 1024;      // candidates that are sorted; at least kMostSlices * kMostTop
+constexpr int kGroups = 8;    // largest values that a sweeping thread leaves of a row
+constexpr int kQueue = 512;   // groups of columns that are looked into
+constexpr int kList = 1024;   // candidates that are ranked
+static_assert(kList >= kMostSlices * kMostTop, "the slices' results are candidates");
 
 // Order of logits as unsigned integers: NaN above everything, both zeros alike.
 __device__ __forceinline__ uint32_t keyOf(float v) {
@@ -28,265 +31,415 @@ __device__ __forceinline__ float valueOf(uint32_t key) {
 // A larger logit, then a smaller column, is the larger entry; no entry is 0.
 __device__ __forceinline__ uint64_t entryOf(float v, int col) { return (uint64_t)keyOf(v) << 32 | (uint32_t)~col; }
 
-struct TopShared {
-  uint4 vec[kKeptVecs];
-  int at[kKeptVecs];
-  uint64_t list[kList];
-  float bound[2][kWarps];
+struct Groups {
+  float top[kGroups][kThreads];
+};
+struct TopWork {
+  alignas(16) uint64_t list[kList];
+  uint64_t best[kMostTop];  // the result, in falling order
   unsigned hist[256];
-  unsigned kept, listed, digit, left;
+  int queue[kQueue];
+  float bound[kWarps];
+  unsigned queued, listed, digit, left;
 };
 
-// Falling order of 32 values, one per lane.
-__device__ __forceinline__ float sortedLanes(float v) {
+// Falling (or rising) order of 32 values, one per lane.
+__device__ __forceinline__ float sortedLanes(float v, bool falling) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
     for (int step = size / 2; step > 0; step /= 2) {
       const float o = __shfl_xor_sync(kAll, v, step);
-      const bool larger = ((lane & step) == 0) == ((lane & size) == 0 || size == 32);
+      const bool larger = ((lane & step) == 0) == ((size == 32 || (lane & size) == 0) == falling);
       v = larger ? fmaxf(v, o) : fminf(v, o);
     }
   return v;
 }
-
-// Keeps the vectors of the sweep that may hold one of the k largest.  If every warp has seen r = ceil(k / warps)
-// values of `bound` or more, one in each of r lanes, k values of the row are that large.  So each warp
-// sorts its lanes' maxima and gives its r-th; the smallest of these is the bound, renewed after batches 1, 2, 4, ...
-// A vector below it is out.  What passes is a few hundred vectors of a row, against 8 compares per logit that
-// picking single logits costs.
-struct TopHook {
-  TopShared* shared;
-  int rank_in_warp;  // r - 1
-  float bound = -INFINITY;
-  int renewals = 0;
-  template <typename V> __device__ __forceinline__ void mask(uint4 (&)[kBatch], int, const V&) {}
-  __device__ __forceinline__ void renew(float top) {
-    float* mine = shared->bound[renewals++ & 1];
-    const float r = __shfl_sync(kAll, sortedLanes(top), rank_in_warp);
-    if ((threadIdx.x & 31) == 0) mine[threadIdx.x >> 5] = r;
-    __syncthreads();
-    float b = mine[0];
+// Falling order of the 32 largest of 64 values, two per lane.
+__device__ __forceinline__ float sortedLanes(float a, float b) {
+  float v = fmaxf(sortedLanes(a, true), sortedLanes(b, false));
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 1; i < kWarps; ++i) b = fminf(b, mine[i]);
-    bound = b;
+  for (int step = 16; step > 0; step /= 2) {
+    const float o = __shfl_xor_sync(kAll, v, step);
+    v = (lane & step) == 0 ? fmaxf(v, o) : fminf(v, o);
   }
-  __device__ __forceinline__ bool passes(float v) const { return v >= bound && v > -INFINITY; }
-  template <typename V>
-  __device__ __forceinline__ void batch(int b, const uint4 (&now)[kBatch], const float (&vmax)[kBatch], float top, int i,
-                                        const V&) {
-    if ((b & (b + 1)) == 0) renew(top);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (passes(vmax[u])) {
-        const unsigned pos = atomicAdd(&shared->kept, 1u);
-        if (pos < kKeptVecs) {
-          shared->vec[pos] = now[u];
-          shared->at[pos] = i + u * kThreads;
-        }
-      }
+  return v;
+}
+
+// While a row is swept every thread leaves the largest value of each of its groups: what it has of one batch, or of `span`
+// batches that follow one another in a row of more than kGroups.
+struct TopHook {
+  Groups* groups;
+  int span, g = 0, in = 0;
+  float top = -INFINITY;
+  template <typename T> static __device__ __forceinline__ int batches(const Slice<T>& sl) {
+    return (sl.v1 - sl.v0 + kBatch * kThreads - 1) / (kBatch * kThreads);
+  }
+  template <typename T> static __device__ __forceinline__ int spanOf(const Slice<T>& sl) {
+    return max(1, (batches(sl) + kGroups - 1) / kGroups);
+  }
+  template <typename T>
+  __device__ __forceinline__ float batch(const uint4 (&now)[kBatch], bool first, int, const Slice<T>& sl) {
+    if (first) span = spanOf(sl);
+    const float largest = batchMax<T>(now);
+    top = fmaxf(top, largest);
+    if (++in == span) {
+      groups->top[g][threadIdx.x] = top;
+      ++g;
+      in = 0;
+      top = -INFINITY;
+    }
+    return largest;
+  }
+  __device__ __forceinline__ void end() {
+    if (in > 0) groups->top[g][threadIdx.x] = top;
   }
 };
 
-// The first `n` entries of the list in falling order; those up to the next power of two are overwritten.
-__device__ __forceinline__ void sortList(uint64_t* list, int n) {
+// The `want` largest of the first n entries of the list, in falling order, to `best`.
+template <class G> __device__ __forceinline__ void rankList(TopWork& work, int n, int want) {
+  uint64_t* list = work.list;
+  if (n <= 2 * G::kSize) {  // every entry counts those above it, two threads an entry where there are threads enough
+    if (G::rank() == 0 && (n & 1)) list[n] = 0;
+    if (n & 1) G::sync();
+    const bool split = 2 * n <= G::kSize;
+    const int pairs = (n + 1) / 2, from = split && (G::rank() & 1) ? pairs / 2 : 0, to = split && !(G::rank() & 1) ? pairs / 2 : pairs;
+    for (int i = split ? G::rank() / 2 : G::rank(); i < (split ? G::kSize / 2 : (n + 31) / 32 * 32); i += G::kSize) {
+      const uint64_t mine = i < n ? list[i] : 0;
+      int above = 0;
+#pragma unroll 4
+      for (int j = from; j < to; ++j) {
+        const ulonglong2 two = reinterpret_cast<const ulonglong2*>(list)[j];
+        above += two.x > mine;
+        above += two.y > mine;
+      }
+      if (split) above += __shfl_xor_sync(kAll, above, 1);
+      if (i < n && above < want) work.best[above] = mine;
+    }
+    G::sync();
+    return;
+  }
   int size = 2;
   while (size < n) size *= 2;
-  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) list[i] = 0;
-  __syncthreads();
+  for (int i = n + G::rank(); i < size; i += G::kSize) list[i] = 0;
+  G::sync();
   for (int block = 2; block <= size; block *= 2)
     for (int step = block / 2; step > 0; step /= 2) {
-      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+      for (int i = G::rank(); i < size / 2; i += G::kSize) {
         const int a = 2 * i - (i & (step - 1)), b = a + step;
         const uint64_t x = list[a], y = list[b];
         if ((x < y) == ((a & block) == 0)) list[a] = y, list[b] = x;
       }
-      __syncthreads();
+      G::sync();
     }
+  for (int i = G::rank(); i < want; i += G::kSize) work.best[i] = list[i];
+  G::sync();
 }
 
-// The `want` largest of the slice's entries, into the list in any order, by a radix select that reads the slice six
-// times and more: for rows where the bound lets too much pass (ties, falling or rising logits) and those with NaN.
-template <typename T> __device__ void selectExactly(const Slice<T>& sl, int want, TopShared* sh) {
+// The `want` largest of the slice's entries, to the list in any order, by a radix select that reads the slice six
+// times and more: for rows where the bound lets too much pass (ties, rising logits) and those with NaN.
+template <class G, typename T> __device__ __noinline__ void selectExactly(const Slice<T>& sl, int want, TopWork& work) {
+  const int tid = G::rank(), lane = threadIdx.x & 31;
   uint32_t prefix = 0;
   unsigned left = want;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    sh->hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int col = sl.c0 + (int)threadIdx.x; col < sl.c1; col += kThreads) {
+    for (int i = tid; i < 256; i += G::kSize) work.hist[i] = 0;
+    G::sync();
+    for (int col = sl.c0 + tid; col < sl.c1; col += G::kSize) {
       const uint32_t key = keyOf(toFloat(sl.row[col]));
-      if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&sh->hist[key >> shift & 255u], 1u);
+      if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&work.hist[key >> shift & 255u], 1u);
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
+    G::sync();
+    if (tid == 0) {
       int digit = 255;
       unsigned more = left;
-      while (digit > 0 && sh->hist[digit] < more) more -= sh->hist[digit--];
-      sh->digit = digit;
-      sh->left = more;
+      while (digit > 0 && work.hist[digit] < more) more -= work.hist[digit--];
+      work.digit = digit;
+      work.left = more;
     }
-    __syncthreads();
-    prefix = prefix << 8 | sh->digit;
-    left = sh->left;
-    __syncthreads();
+    G::sync();
+    prefix = prefix << 8 | work.digit;
+    left = work.left;
+    G::sync();
   }
   // `prefix` is the key of the last one; `left` of those that equal it are taken, the first ones.
-  if (threadIdx.x == 0) sh->listed = 0;
-  __syncthreads();
-  for (int col = sl.c0 + (int)threadIdx.x; col < sl.c1; col += kThreads) {
+  if (tid == 0) work.listed = 0;
+  G::sync();
+  for (int col = sl.c0 + tid; col < sl.c1; col += G::kSize) {
     const float v = toFloat(sl.row[col]);
-    if (keyOf(v) > prefix) sh->list[atomicAdd(&sh->listed, 1u)] = entryOf(v, col);
+    if (keyOf(v) > prefix) work.list[atomicAdd(&work.listed, 1u)] = entryOf(v, col);
   }
   const unsigned larger = want - left;
   unsigned taken = 0;
-  for (int base = sl.c0; base < sl.c1 && taken < left; base += kThreads) {
-    const int col = base + (int)threadIdx.x;
+  for (int base = sl.c0; base < sl.c1 && taken < left; base += G::kSize) {
+    const int col = base + tid;
     const float v = col < sl.c1 ? toFloat(sl.row[col]) : 0.f;
     const bool equal = col < sl.c1 && keyOf(v) == prefix;
     const unsigned votes = __ballot_sync(kAll, equal);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh->hist[threadIdx.x >> 5] = __popc(votes);
-    __syncthreads();
-    unsigned before = taken + __popc(votes & ((1u << (threadIdx.x & 31)) - 1u)), all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < (int)(threadIdx.x >> 5)) before += sh->hist[w];
-      all += sh->hist[w];
+    G::sync();
+    if (lane == 0) work.hist[tid >> 5] = __popc(votes);
+    G::sync();
+    unsigned before = taken + __popc(votes & ((1u << lane) - 1u)), all = 0;
+    for (int w = 0; w < G::kSize / 32; ++w) {
+      if (w < tid >> 5) before += work.hist[w];
+      all += work.hist[w];
     }
-    if (equal && before < left) sh->list[larger + before] = entryOf(v, col);
+    if (equal && before < left) work.list[larger + before] = entryOf(v, col);
     taken += all;
   }
-  __syncthreads();
+  G::sync();
 }
 
-// The slice's largest entries, at most k, in falling order at the start of the list; zeros behind them up to k.
-template <typename T>
-__device__ void sliceTop(const Slice<T>& sl, int k, float top, bool nan, TopHook& hook, TopShared* sh) {
-  constexpr int E = Vec<T>::kElems;
-  const int want = min(k, sl.c1 - sl.c0);
-  hook.renew(top);
-  const unsigned kept = sh->kept;
-  if (kept <= kKeptVecs) {
-    for (unsigned j = threadIdx.x; j < kept; j += kThreads) {
-      float2 v[E / 2];
-      Vec<T>::get(sh->vec[j], v);
-      const int col = sl.head + sh->at[j] * E;
+// The slice's largest entries, at most k, in falling order, to `best`, zeros behind them up to k.  The sweep is over for all of the
+// group, and work.queued and work.listed are 0; they are 0 again afterwards.
+//
+// If each of the group's w warps finds r = ceil(k / w) values of `bound` or more among the largest values of the sweep's columns of
+// threads, k values of the slice are that large: each warp sorts what it has of those and gives its r-th, and the smallest
+// of these is the bound.  Groups below it are out, a hundred or two of the 2048 are looked into again, and what they have above the
+// bound, again a hundred or two values, is ranked.
+template <class G, typename T>
+__device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, const Groups& groups, TopWork& work) {
+  constexpr int E = Vec<T>::kElems, kColumns = kThreads / G::kSize, kGroupWarps = G::kSize / 32;
+  static_assert(kColumns == 1 || kColumns == 2, "columns of threads that a thread looks at");
+  const int tid = G::rank(), lane = threadIdx.x & 31, want = min(k, sl.c1 - sl.c0);
+  const int batches = TopHook::batches(sl), span = TopHook::spanOf(sl), number = (batches + span - 1) / span;
+  float value[kGroups * kColumns], top[kColumns];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float x = e & 1 ? v[e / 2].y : v[e / 2].x;
-        if (hook.passes(x)) {
-          const unsigned pos = atomicAdd(&sh->listed, 1u);
-          if (pos < kList) sh->list[pos] = entryOf(x, col + e);
-        }
-      }
+  for (int j = 0; j < kColumns; ++j) {
+    top[j] = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      value[j * kGroups + g] = g < number ? groups.top[g][tid + j * G::kSize] : -INFINITY;
+      top[j] = fmaxf(top[j], value[j * kGroups + g]);
     }
-    const int col = threadIdx.x < 2 * E ? sl.looseCol(threadIdx.x) : -1;
-    if (col >= 0) {
-      const float x = toFloat(sl.row[col]);
-      if (hook.passes(x)) {
-        const unsigned pos = atomicAdd(&sh->listed, 1u);
-        if (pos < kList) sh->list[pos] = entryOf(x, col);
+  }
+  const float sorted = kColumns == 1 ? sortedLanes(top[0], true) : sortedLanes(top[0], top[kColumns - 1]);
+  const float mine = __shfl_sync(kAll, sorted, (k + kGroupWarps - 1) / kGroupWarps - 1);
+  if (lane == 0) work.bound[tid >> 5] = mine;
+  G::sync();
+  float bound = work.bound[0];
+#pragma unroll
+  for (int w = 1; w < kGroupWarps; ++w) bound = fminf(bound, work.bound[w]);
+  bound = fmaxf(bound, -FLT_MAX);  // minus infinity is left to the other way
+#pragma unroll
+  for (int j = 0; j < kColumns; ++j)
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const bool pass = value[j * kGroups + g] >= bound;
+      const unsigned votes = __ballot_sync(kAll, pass);
+      if (votes == 0) continue;
+      unsigned pos = 0;
+      if (lane == 0) pos = atomicAdd(&work.queued, (unsigned)__popc(votes));
+      pos = __shfl_sync(kAll, pos, 0) + __popc(votes & ((1u << lane) - 1u));
+      if (pass && pos < kQueue) work.queue[pos] = g * kThreads + tid + j * G::kSize;
+    }
+  G::sync();
+  const int queued = work.queued, vecs_each = kBatch * span;
+  const bool fits = queued <= kQueue;
+  const uint4* all = reinterpret_cast<const uint4*>(sl.row + sl.head);
+  constexpr int kAhead = 4;
+  const int items = fits ? queued * vecs_each : 0;
+  for (int first = 0; first < items; first += kAhead * G::kSize) {
+    uint4 raw[kAhead];
+    int at[kAhead];
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      const int j = first + s * G::kSize + tid;
+      at[s] = sl.v1;
+      if (j < items) {
+        const int id = work.queue[j / vecs_each];
+        at[s] = sl.v0 + id / kThreads * vecs_each * kThreads + j % vecs_each * kThreads + id % kThreads;
+      }
+      constexpr uint32_t w = Vec<T>::kMinusInf;
+      raw[s] = at[s] < sl.v1 ? all[at[s]] : make_uint4(w, w, w, w);  // swept not long ago: from L2
+    }
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+      if (first + s * G::kSize >= items) break;
+      float2 v[E / 2];
+      Vec<T>::get(raw[s], v);
+      unsigned mask = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) mask |= (e & 1 ? v[e / 2].y : v[e / 2].x) >= bound ? 1u << e : 0u;
+      for (;;) {  // a value of every lane that has one
+        const unsigned votes = __ballot_sync(kAll, mask != 0);
+        if (votes == 0) break;
+        unsigned pos = 0;
+        if (lane == 0) pos = atomicAdd(&work.listed, (unsigned)__popc(votes));
+        pos = __shfl_sync(kAll, pos, 0) + __popc(votes & ((1u << lane) - 1u));
+        if (mask != 0 && pos < kList) {
+          const int col = sl.head + at[s] * E + __ffs(mask) - 1;
+          work.list[pos] = entryOf(toFloat(sl.row[col]), col);
+        }
+        mask &= mask - 1;
       }
     }
   }
-  __syncthreads();
-  int n = sh->listed;
-  __syncthreads();
-  if (nan || kept > kKeptVecs || n > kList || n < want) {
-    selectExactly(sl, want, sh);
+  const int loose = tid < 2 * E ? sl.looseCol(tid) : -1;
+  if (loose >= 0) {
+    const float v = toFloat(sl.row[loose]);
+    const unsigned pos = v >= bound ? atomicAdd(&work.listed, 1u) : kList;
+    if (pos < kList) work.list[pos] = entryOf(v, loose);
+  }
+  G::sync();
+  int n = work.listed;
+  G::sync();
+  if (nan || !fits || n > kList || n < want) {
+    if (want > 0) selectExactly<G>(sl, want, work);
     n = want;
   }
-  sortList(sh->list, max(n, 1));
-  for (int i = max(n, 1) + (int)threadIdx.x; i < k; i += kThreads) sh->list[i] = 0;
-  if (n == 0 && threadIdx.x == 0) sh->list[0] = 0;
-  __syncthreads();
+  if (tid == 0) work.listed = work.queued = 0;
+  for (int i = want + tid; i < k; i += G::kSize) work.best[i] = 0;
+  rankList<G>(work, n, want);
 }
 
-// The k largest of the row from the slices' lists, in block 0.  clusterSums() has waited for the lists.
-__device__ __forceinline__ void clusterTop(int k, TopShared* sh) {
+// The k largest of the row from the slices' results, in block 0.  clusterSums() has waited for those.
+__device__ __forceinline__ void clusterTop(int k, TopWork& work) {
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.num_blocks();
-  if (slices == 1 || cluster.block_rank() != 0) return;
-  for (int i = threadIdx.x; i < (slices - 1) * k; i += kThreads) {
-    const int r = 1 + i / k;
-    sh->list[r * k + (i - (r - 1) * k)] = cluster.map_shared_rank(sh, r)->list[i - (r - 1) * k];
+  if (cluster.block_rank() != 0) return;
+  for (int i = threadIdx.x; i < slices * k; i += kThreads) {
+    const int r = i / k;
+    work.list[i] = cluster.map_shared_rank(&work, r)->best[i - r * k];
   }
   __syncthreads();
-  sortList(sh->list, slices * k);
+  rankList<BlockGroup>(work, slices * k, k);
 }
 
-// One row per cluster.  Kept for the backward: the row's maximum and S; S is -1 where the row does not count
-// and NaN where its token is none.
+// What one row leaves; any pointer but `tokens` may be null.  Kept for the backward: m and S as its exponents need it, which is
+// -1 where the row does not count and NaN where its token is none.
+struct Outputs {
+  const int64_t* tokens;
+  float* log_probs;
+  float* entropy;
+  float2* stats;
+  int k;
+  float* top_log_probs;
+  int64_t* top_tokens;
+
+  __device__ __forceinline__ void skipped(int64_t r) const {  // by one thread
+    if (log_probs != nullptr) log_probs[r] = 0.f;
+    if (entropy != nullptr) entropy[r] = 0.f;
+    if (stats != nullptr) stats[r] = make_float2(0.f, -1.f);
+    for (int i = 0; i < k; ++i) {
+      top_log_probs[r * k + i] = -INFINITY;
+      top_tokens[r * k + i] = -1;
+    }
+  }
+  // By one thread; `logit` is the token's.
+  template <bool kEntropy>
+  __device__ __forceinline__ void values(int64_t r, const Sums& acc, bool known, float logit, float c, float inv_t) const {
+    const float low = logf(acc.s), nan = __int_as_float(0x7fffffff);
+    if (log_probs != nullptr) log_probs[r] = known ? fmaf(logit - acc.m, inv_t, -low) : nan;
+    if (kEntropy) entropy[r] = low - acc.a / acc.s * kLn2;
+    if (stats != nullptr) stats[r] = make_float2(acc.m, known ? acc.s * exp2Of(Exponent::excess(acc.m, c)) : nan);
+  }
+  template <class G>
+  __device__ __forceinline__ void largest(int64_t r, const Sums& acc, const uint64_t* best, float inv_t) const {
+    const float low = logf(acc.s);
+    for (int i = G::rank(); i < k; i += G::kSize) {
+      const uint64_t entry = best[i];
+      top_log_probs[r * k + i] = fmaf(valueOf((uint32_t)(entry >> 32)) - acc.m, inv_t, -low);
+      top_tokens[r * k + i] = (int)~(uint32_t)entry;
+    }
+  }
+};
+
+struct TopSlices {
+  TopWork work;
+  Groups groups;
+};
+
+// Few rows: one per cluster.
 template <typename T, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kThreads, kTop ? 3 : 4)
-token_log_probs_fwd_kernel(const T* __restrict__ logits, LogitRows x, const int64_t* __restrict__ tokens, float c,
-                           float inv_t, float* __restrict__ log_probs, float* __restrict__ entropy,
-                           float2* __restrict__ stats, int k, float* __restrict__ top_log_probs,
-                           int64_t* __restrict__ top_tokens) {
+token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t) {
   namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ Sums scratch[kWarps], mine;
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.num_blocks(), rank = cluster.block_rank();
   const int64_t r = blockIdx.x / slices;
-  const int64_t t = tokens != nullptr ? tokens[r] : 0;
+  const int64_t t = out.tokens != nullptr ? out.tokens[r] : 0;
   if (t < 0) {
-    if (rank != 0) return;
-    if (threadIdx.x == 0) {
-      if (log_probs != nullptr) log_probs[r] = 0.f;
-      if (kEntropy) entropy[r] = 0.f;
-      if (stats != nullptr) stats[r] = make_float2(0.f, -1.f);
-    }
-    if (kTop)
-      for (int i = threadIdx.x; i < k; i += kThreads) {
-        top_log_probs[r * k + i] = -INFINITY;
-        top_tokens[r * k + i] = -1;
-      }
+    if (rank == 0 && threadIdx.x == 0) out.skipped(r);
     return;
   }
   const Slice<T> sl(rowOf(x, logits, r), x.vocab, rank, slices);
+  const bool known = t < x.vocab;
+  float logit = 0.f;
+  if (rank == 0 && threadIdx.x == 0 && known) logit = toFloat(sl.row[t]);
   Sums acc;
-  TopShared* sh = nullptr;
-  TopHook hook;
+  TopSlices* top = reinterpret_cast<TopSlices*>(dynamic);
   if constexpr (kTop) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
-    sh = reinterpret_cast<TopShared*>(dynamic);
-    hook.shared = sh;
-    hook.rank_in_warp = (k + kWarps - 1) / kWarps - 1;
-    if (threadIdx.x == 0) sh->kept = sh->listed = 0;
-    __syncthreads();
+    TopHook hook;
+    hook.groups = &top->groups;
+    if (threadIdx.x == 0) top->work.listed = top->work.queued = 0;
     acc = scan<T, kEntropy>(sl, c, hook);
+    hook.end();
   } else {
     NoHook none;
     acc = scan<T, kEntropy>(sl, c, none);
   }
-  const float top = acc.m;
   if (threadIdx.x < 2 * Vec<T>::kElems) {
     const int col = sl.looseCol(threadIdx.x);
     if (col >= 0) acc.add<kEntropy>(toFloat(sl.row[col]), c);
   }
   acc = blockSums<kEntropy>(acc, c, scratch);
-  if constexpr (kTop) sliceTop(sl, k, top, acc.s != acc.s, hook, sh);
+  if constexpr (kTop) sliceTop<BlockGroup>(sl, out.k, acc.s != acc.s, top->groups, top->work);
   if (slices > 1) {
     acc = clusterSums<kEntropy>(acc, c, &mine);
-    if constexpr (kTop) clusterTop(k, sh);
+    if constexpr (kTop) clusterTop(out.k, top->work);
     clusterDone();
     if (rank != 0) return;
   }
-  const float low = logf(acc.s);
-  if (threadIdx.x == 0) {
-    const bool known = t < x.vocab;
-    if (log_probs != nullptr)
-      log_probs[r] = known ? fmaf(toFloat(sl.row[t]) - acc.m, inv_t, -low) : __int_as_float(0x7fffffff);
-    if (kEntropy) entropy[r] = low - acc.a / acc.s * kLn2;
-    if (stats != nullptr) stats[r] = make_float2(acc.m, known ? acc.s : __int_as_float(0x7fffffff));
+  if (!acc.template settle<kEntropy>(c)) acc = blockAgain<T, kEntropy>(sl.row, x.vocab, c, scratch, LeaveNone());
+  if (threadIdx.x == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
+  if constexpr (kTop) out.largest<BlockGroup>(r, acc, top->work.best, inv_t);
+}
+
+// Many rows: the blocks stay.
+constexpr int kFinishers = 64, kUnfinished = 4;
+struct Rows {
+  Ring ring;
+  HandOver<kUnfinished> hand;
+};
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(kThreads + kFinishers, 3)
+token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  Rows& shared = *reinterpret_cast<Rows*>(dynamic);
+  HandOver<kUnfinished>& hand = shared.hand;
+  if (threadIdx.x == 0) hand.init();
+  __syncthreads();
+  const int64_t* tokens = out.tokens;
+  const auto counts = [tokens](int r) { return tokens == nullptr || tokens[r] >= 0; };
+  if (threadIdx.x < kThreads) {
+    NoHook none;
+    sweepRows<T, kEntropy>(logits, x, counts, c, shared.ring, hand, none);
+    return;
   }
-  if constexpr (kTop)
-    for (int i = threadIdx.x; i < k; i += kThreads) {
-      const uint64_t entry = sh->list[i];
-      top_log_probs[r * k + i] = fmaf(valueOf((uint32_t)(entry >> 32)) - acc.m, inv_t, -low);
-      top_tokens[r * k + i] = (int)~(uint32_t)entry;
-    }
+  const int which = (int)(threadIdx.x - kThreads) / 32, lane = threadIdx.x & 31;
+  const auto finish = [&](int64_t r, int buffer, unsigned parity) {
+    const Slice<T> sl(rowOf(x, logits, r), x.vocab, 0, 1);
+    const int64_t t = tokens != nullptr ? tokens[r] : 0;
+    const bool known = t < x.vocab;
+    const float logit = known ? toFloat(sl.row[t]) : 0.f;
+    hand.wait(&hand.full[buffer], parity);
+    Sums acc = hand.template take<T, kEntropy>(buffer, sl, c, 0);
+    __syncwarp();
+    if (lane == 0) barrierArrive(&hand.empty[buffer]);
+    if (!acc.template settle<kEntropy>(c)) acc = warpAgain<T, kEntropy>(sl.row, x.vocab, c, LeaveNone());
+    if (hand.gaveUp()) acc.s = __int_as_float(0x7fffffff);
+    if (lane != 0) return;
+    out.values<kEntropy>(r, acc, known, logit, c, inv_t);
+  };
+  finishRows<kUnfinished>(counts, x.rows, which, kFinishers / 32, finish, [&](int64_t r) {
+    if (which == 0) out.skipped(r);
+  });
 }
 
 // A block does one batch of vectors of one row, so that all blocks are alike whatever the vocabulary.
@@ -320,9 +473,9 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restr
     // g (1[v = t] - p) - h p (log p + H) with p = e / S and log p = u ln 2 - log S, u the exponent of e
     const float per_s = 1.f / st.y;
     const float a = -(kEntropy ? fmaf(h, entropy[r] - logf(st.y), g) : g) * per_s, b = -h * kLn2 * per_s;
+    const Exponent exponent(st.x, c);
     auto of = [&](float2 v) {
-      const float2 d = mul2(add2(v, make_float2(-st.x, -st.x)), make_float2(c, c));
-      const float2 e = make_float2(exp2Of(d.x), exp2Of(d.y));
+      const float2 d = exponent(v), e = make_float2(exp2Of(d.x), exp2Of(d.y));
       if (!kEntropy) return mul2(e, make_float2(a, a));
       return mul2(e, fma2(make_float2(fmaxf(d.x, kLowExponent), fmaxf(d.y, kLowExponent)), make_float2(b, b), make_float2(a, a)));
     };
@@ -356,18 +509,25 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restr
   }
 }
 
+template <typename T, bool kEntropy>
+cudaError_t forwardOf(const T* logits, const LogitRows& x, const Outputs& out, double temperature, int sm_count, cudaStream_t stream) {
+  const float inv_t = (float)(1.0 / temperature), c = (float)(1.4426950408889634 / temperature);
+  if (out.k == 0 && manyRows(x.rows, sm_count))
+    return launchResident(token_log_probs_rows_kernel<T, kEntropy>, x.rows, kThreads + kFinishers, 3, sizeof(Rows), sm_count,
+                          stream, logits, x, out, c, inv_t);
+  const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
+  if (out.k > 0)
+    return launchSlices(token_log_probs_slices_kernel<T, kEntropy, true>, x.rows, slices,
+                        sizeof(TopSlices), stream, logits, x, out, c, inv_t);
+  return launchSlices(token_log_probs_slices_kernel<T, kEntropy, false>, x.rows, slices, 0, stream, logits, x, out, c, inv_t);
+}
+
 template <typename T>
 cudaError_t forwardOf(const void* logits, const LogitRows& x, const TokenLogProbsArgs& a, int sm_count, cudaStream_t stream) {
-  const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
+  const Outputs out{a.tokens, a.log_probs, a.entropy, reinterpret_cast<float2*>(a.stats), a.k, a.top_log_probs, a.top_tokens};
   const T* data = static_cast<const T*>(logits);
-  const float inv_t = (float)(1.0 / a.temperature), c = (float)(1.4426950408889634 / a.temperature);
-  const size_t shared = a.k > 0 ? sizeof(TopShared) : 0;
-  auto run = [&](auto kernel) {
-    return launchSlices(kernel, x.rows, slices, shared, stream, data, x, a.tokens, c, inv_t, a.log_probs, a.entropy,
-                        reinterpret_cast<float2*>(a.stats), a.k, a.top_log_probs, a.top_tokens);
-  };
-  if (a.k > 0) return a.entropy != nullptr ? run(token_log_probs_fwd_kernel<T, true, true>) : run(token_log_probs_fwd_kernel<T, false, true>);
-  return a.entropy != nullptr ? run(token_log_probs_fwd_kernel<T, true, false>) : run(token_log_probs_fwd_kernel<T, false, false>);
+  return a.entropy != nullptr ? forwardOf<T, true>(data, x, out, a.temperature, sm_count, stream)
+                              : forwardOf<T, false>(data, x, out, a.temperature, sm_count, stream);
 }
 
 template <typename T>

@@ -79,6 +79,18 @@ def test_every_row_length(rows, vocab, k, rest, dtype):
         assert loss[2] == 0 and not grad[2].any()
 
 
+# rows that are taken by blocks that stay
+@pytest.mark.parametrize("vocab,k", [(7, 3), (264, 256), (1001, 5), (8193, 64), (20011, 33)])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows(vocab, k, rest, dtype):
+    x, tokens, given = _case(1300, vocab, k, dtype)
+    tokens[100:900] = -1  # most blocks have rows that do not count
+    tokens[950:1000, 1:] = tokens[950:1000, :1]  # one token all over
+    tokens[1299, :-1] = -1  # only the last entry
+    _check(x, tokens, given - 0.2 if rest else given, 1.3, rest)
+
+
 @pytest.mark.parametrize("temperature", [0.5, 2.0])
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -226,11 +238,12 @@ def test_second_derivative(rest, reduction):
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6)
 
 
-def test_bits_repeat_and_modes():
+@pytest.mark.parametrize("rows", [40, 1350])
+def test_bits_repeat_and_modes(rows):
     from fairring_b200 import launch_count
     from fairring_b200.ops import distillation_loss
 
-    x, tokens, given = _case(40, 50265, 64, torch.bfloat16)
+    x, tokens, given = _case(rows, 50265, 64, torch.bfloat16)
     tokens[:, 3] = tokens[:, 0]
     for rest in (False, True):
         got = []

@@ -61,8 +61,8 @@ def _check(logits, tokens, temperature=1.0, entropy=True):
 
 
 # one thread's worth, remainders on both sides of the 16-byte vectors, one batch of a block (256 x 4 vectors) and the
-# next; 19 rows are cut into slices from 512 vectors a slice on, 400 rows are not
-@pytest.mark.parametrize("rows", [1, 19, 400])
+# next; 19 rows are cut into slices from 512 vectors a slice on, 400 rows are not; 1300 rows are taken by blocks that stay
+@pytest.mark.parametrize("rows", [1, 19, 400, 1300])
 @pytest.mark.parametrize("vocab", [1, 7, 8, 9, 1000, 1001, 4096, 8191, 8192, 8193, 16385, 32776, 50265])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_every_row_length(rows, vocab, dtype):
@@ -83,7 +83,7 @@ def test_temperature(temperature, entropy, dtype):
     _check(logits, torch.randint(0, 5003, (37,), device="cuda", generator=_gen(2)), temperature, entropy)
 
 
-@pytest.mark.parametrize("rows,vocab", [(3, 1001), (3, 50265), (300, 20000)])
+@pytest.mark.parametrize("rows,vocab", [(3, 1001), (3, 50265), (300, 20000), (1301, 1001), (1301, 20000)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_masked_logits(rows, vocab, dtype):
     """Minus infinity and the type's lowest value, up to rows of nothing else."""
@@ -115,7 +115,7 @@ def test_masked_logits(rows, vocab, dtype):
     assert bool(grad[1].isnan().all()) and bool(grad[0].isfinite().all()) and bool(grad[2:].isfinite().all())
 
 
-@pytest.mark.parametrize("rows", [6, 320])
+@pytest.mark.parametrize("rows", [6, 320, 1400])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_values_that_are_no_numbers(rows, dtype):
     """NaN and infinity make their own row NaN and no other; a row that does not count may hold anything."""
@@ -156,7 +156,7 @@ def _check_top(logits, k, temperature=1.0):
     assert bool((off <= 2.0 ** -17.3 + 4 * 2.0 ** -24 * want.abs())[fine].all())
 
 
-@pytest.mark.parametrize("rows", [1, 7, 60, 330])
+@pytest.mark.parametrize("rows", [1, 7, 60, 330, 1250])
 @pytest.mark.parametrize("vocab,k", [(1, 1), (5, 5), (130, 128), (1000, 7), (1024, 128), (8193, 1), (32003, 20), (51200, 64),
                                      (50265, 128)])
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -164,7 +164,7 @@ def test_top(rows, vocab, k, dtype):
     _check_top(_logits(rows, vocab, dtype), k, 0.7)
 
 
-@pytest.mark.parametrize("rows", [2, 310])
+@pytest.mark.parametrize("rows", [2, 310, 1201])
 @pytest.mark.parametrize("vocab", [300, 9001, 51200])
 @pytest.mark.parametrize("kind", ["equal", "few values", "rising", "falling", "in one place", "few left", "zeros", "scattered left"])
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -206,6 +206,24 @@ def test_views():
                 assert t.shape == x.shape[:-1]
                 _check(x, t)
     _check(_logits(1, 1003, torch.float32)[0], torch.tensor(5, device="cuda"))  # one row without a leading dimension
+
+
+@pytest.mark.parametrize("share", [0.0, 0.02, 0.5, 0.99, 1.0])
+def test_rows_that_do_not_count_among_many(share):
+    """Whole runs of 32 rows of a block without one that counts, and the last rows of all."""
+    from fairring_b200.ops import token_log_probs
+
+    rows, vocab = 20000, 264
+    gen = _gen(8)
+    logits = _logits(rows, vocab, torch.float32)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
+    tokens[torch.rand(rows, device="cuda", generator=gen) < share] = -100
+    tokens[:5000] = -1
+    logits[tokens < 0] = float("nan")
+    _check(logits.nan_to_num(), tokens)
+    got = token_log_probs(logits, tokens, entropy=True, top_k=3)
+    assert bool(got.entropy.isfinite().all()) and bool((got.top_tokens[tokens < 0] == -1).all())
+    assert torch.equal(got.top_tokens[tokens >= 0], logits[tokens >= 0].sort(dim=1, descending=True, stable=True).indices[:, :3])
 
 
 def test_kinds_of_gradients():
@@ -279,12 +297,13 @@ def test_second_derivative():
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
 
 
-def test_bits_repeat_and_modes():
+@pytest.mark.parametrize("rows", [40, 1350])
+def test_bits_repeat_and_modes(rows):
     from fairring_b200 import launch_count
     from fairring_b200.ops import token_log_probs
 
-    x = _logits(40, 50265, torch.bfloat16)
-    tokens = torch.randint(0, 50265, (40,), device="cuda", generator=_gen(7))
+    x = _logits(rows, 50265, torch.bfloat16)
+    tokens = torch.randint(0, 50265, (rows,), device="cuda", generator=_gen(7))
     first = token_log_probs(x, tokens, entropy=True, top_k=50)
     for _ in range(5):
         for a, b in zip(first, token_log_probs(x, tokens, entropy=True, top_k=50)):
@@ -294,9 +313,10 @@ def test_bits_repeat_and_modes():
         again = token_log_probs(x, tokens, entropy=True, top_k=50)
     assert launch_count() == before + 1
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+    alone = token_log_probs(x, tokens).log_probs  # not the same kernel: its sums are in another order
     with torch.autocast("cuda", dtype=torch.bfloat16):
-        assert torch.equal(token_log_probs(x, tokens).log_probs, first.log_probs)
-    assert torch.equal(token_log_probs(x, tokens.int()).log_probs, first.log_probs)
+        assert torch.equal(token_log_probs(x, tokens).log_probs, alone)
+    assert torch.equal(token_log_probs(x, tokens.int()).log_probs, alone)
 
 
 def test_empty_and_refused():
@@ -321,7 +341,7 @@ def test_empty_and_refused():
     assert bool(g[1].isnan().all()) and bool(g[0].isfinite().all())
 
 
-@pytest.mark.parametrize("rows", [1, 64])
+@pytest.mark.parametrize("rows", [1, 64, 1200])
 def test_streams_and_graphs(rows):
     """Two captured calls with their own inputs, replayed in turn and on another stream."""
     from fairring_b200.ops import token_log_probs
