@@ -17,12 +17,29 @@ using namespace softmax_row;
 // What the teacher says of one row, and the student of the tokens that it names.
 struct Teacher {
   alignas(16) int token[kMostTeacherTokens];  // -1: padding or no token
-  float given[kMostTeacherTokens];            // the teacher's value
-  float logit[kMostTeacherTokens];            // the student's
   float q[kMostTeacherTokens];
+  float logit[kMostTeacherTokens];
   bool first[kMostTeacherTokens];  // no entry before it names the same token
-  double log_total;                // what turns the values into log probabilities
-  double mass;                     // sum of q
+  float log_terms, total;          // sum of q log q is the first less the mass's share of log(total)
+  bool outside;                    // a token is past the vocabulary
+};
+
+// What of the loss needs no sums: of the listed tokens sum q (log q + log total), the sum of q (x - ref), that of q, and with the
+// rest the maximum and the sum of their own exponentials.  A divergence is a small difference of large logarithms: sums are taken of
+// differences to the largest, and what those leave out is put together in 64 bits.
+struct Listed {
+  float log_terms, total, ref, from_ref, mass, m, s;
+};
+
+// Whether the bit was set before.
+__device__ __forceinline__ bool setBit(unsigned* bits, unsigned at) {
+  return atomicOr(&bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u;
+}
+
+struct Given {
+  const int64_t* tokens;
+  const float* log_probs;
+  int k;
 };
 
 // The columns that the sweep leaves out, for a second look at a row.
@@ -54,12 +71,6 @@ template <typename T> struct Marks {
     return (v / (kBatch * kThreads) * kThreads + v % kThreads) * kBits + v / kThreads % kBatch * E + e;
   }
 };
-// Whether the bit was set before.
-__device__ __forceinline__ bool setBit(unsigned* bits, unsigned at) {
-  return atomicOr(&bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u;
-}
-__device__ __forceinline__ void clearBit(unsigned* bits, unsigned at) { atomicAnd(&bits[at >> 5], ~(1u << (at & 31))); }
-
 struct RestHook {
   const unsigned* bits;
   // Those of what this thread has of batch b.
@@ -88,119 +99,152 @@ struct RestHook {
   }
 };
 
-// The entries of row r, by one warp; returns whether one is past the vocabulary.  Then the student's logits of those tokens.
-__device__ __forceinline__ bool loadTeacher(Teacher& te, const int64_t* tokens, const float* log_probs, int k, int64_t r,
-                                            int vocab) {
-  const int lane = threadIdx.x & 31;
-  bool outside = false;
-#pragma unroll 4
-  for (int i = lane; i < k; i += 32) {
-    const int64_t t = tokens[r * k + i];
-    te.given[i] = log_probs[r * k + i];
-    te.token[i] = t < 0 || t >= vocab ? -1 : (int)t;
-    outside |= t >= vocab;
+// Whether a row counts, by one warp: one does that has a listed token and, without the rest, one that the teacher gives some
+// probability.
+template <bool kRest> __device__ __forceinline__ bool countsAtAll(const Given& given, int64_t r) {
+  bool some = false;
+  for (int first = 0; first < given.k && !some; first += 32) {
+    const int i = first + (threadIdx.x & 31);
+    some = i < given.k && given.tokens[r * given.k + i] >= 0 && (kRest || !(given.log_probs[r * given.k + i] == -INFINITY));
+    some = __any_sync(kAll, some);
   }
-  if (lane < 4 && k + lane < kMostTeacherTokens) te.token[k + lane] = -2;
-  __syncwarp();
-  return __any_sync(kAll, outside);
+  return some;
 }
-template <typename T> __device__ __forceinline__ void loadLogits(Teacher& te, int k, const T* row) {
-#pragma unroll 4
-  for (int i = threadIdx.x & 31; i < k; i += 32) te.logit[i] = te.token[i] >= 0 ? toFloat(row[te.token[i]]) : 0.f;
+
+// The entries of row r, the teacher's probabilities and the student's logits, by one warp.
+template <typename T, bool kRest>
+__device__ __forceinline__ void loadTeacher(Teacher& te, const Given& given, int64_t r, const T* row, int vocab, float inv_t) {
+  const int lane = threadIdx.x & 31, k = given.k;
+  bool outside = false;
+  float top = -INFINITY, total = 0.f, terms = 0.f;
+#pragma unroll 2
+  for (int i = lane; i < k; i += 32) {
+    const int64_t t = given.tokens[r * k + i];
+    const float value = given.log_probs[r * k + i];
+    const bool known = t >= 0 && t < vocab;
+    outside |= t >= vocab;
+    te.token[i] = known ? (int)t : -1;
+    te.q[i] = known ? value : -INFINITY;
+    te.logit[i] = known ? toFloat(row[t]) : 0.f;
+    if (known) top = fmaxf(top, value);
+  }
+  if (lane < 4 && k + lane < kMostTeacherTokens) te.token[k + lane] = -2;  // behind the last: no token
+  outside = __any_sync(kAll, outside);
+  top = kRest ? 0.f : warpMax(top);
+  if (top == -INFINITY) top = 0.f;
+  const float scale = kRest ? 1.f : inv_t;
+  // What is stored becomes the exponential, which is divided by the total when that is known.
+  for (int i = lane; i < k; i += 32) {
+    const float d = (te.q[i] - top) * scale, e = expf(d);
+    te.q[i] = e;
+    total += e;
+    if (!(e == 0.f)) terms = fmaf(e, d, terms);
+  }
+  terms = warpSum(terms);
+  float per_total = 1.f;
+  if constexpr (!kRest) {
+    total = warpSum(total);
+    per_total = 1.f / total;
+    for (int i = lane; i < k; i += 32) te.q[i] *= per_total;
+  }
+  if (lane == 0) te.log_terms = terms * per_total, te.total = kRest ? 1.f : total, te.outside = outside;
   __syncwarp();
 }
 
-// The teacher's probabilities, and with `merged` the listed tokens, each once, with the sum of what its entries
-// have, by one warp.  `twice`: a token may be named more than once.
-template <bool kRest> __device__ __forceinline__ void teacherOf(Teacher& te, int k, float inv_t, bool twice, int2* merged) {
+// Whether a token is named more than once, by one warp.  Its bit is that of its number's end: where another token had set it, that
+// token is looked for among all.  `bits`: kNameWords of zeros, as they are again afterwards.
+constexpr int kNameWords = 1024;
+__device__ __forceinline__ bool namedTwice(const Teacher& te, int k, unsigned* bits) {
   const int lane = threadIdx.x & 31;
-  if constexpr (kRest) {
-    double mass = 0;
-    for (int i = lane; i < k; i += 32) {
-      const float q = te.token[i] >= 0 ? expf(te.given[i]) : 0.f;
-      te.q[i] = q;
-      mass += q;
+  bool twice = false;
+  for (int first = 0; first < k; first += 32) {
+    const int i = first + lane, t = i < k ? te.token[i] : -1;
+    const bool set = t >= 0 && setBit(bits, t % (32 * kNameWords));
+    for (unsigned mask = __ballot_sync(kAll, set); mask != 0; mask &= mask - 1) {
+      const int wanted = __shfl_sync(kAll, t, __ffs(mask) - 1);
+      unsigned found = 0;
+      for (int j = lane; j < k; j += 32) found += te.token[j] == wanted;
+      twice |= __reduce_add_sync(kAll, found) > 1;
     }
-    mass = warpSum(mass);
-    if (lane == 0) te.mass = mass, te.log_total = 0;
-  } else {
-    float top = -INFINITY, total = 0.f;
-    for (int i = lane; i < k; i += 32)
-      if (te.token[i] >= 0) top = fmaxf(top, te.given[i]);
-    top = warpMax(top);
-    for (int i = lane; i < k; i += 32) {
-      const float q = te.token[i] >= 0 ? expf((te.given[i] - top) * inv_t) : 0.f;
-      te.q[i] = q;
-      total += q;
-    }
-    total = warpSum(total);
-    for (int i = lane; i < k; i += 32) te.q[i] /= total;
-    if (lane == 0) te.mass = 1, te.log_total = (double)top * inv_t + log((double)total);
   }
   __syncwarp();
-  if (!kRest && merged == nullptr) return;
-  if (!twice) {
-    for (int i = lane; i < k; i += 32) {
-      te.first[i] = te.token[i] >= 0;
-      if (merged != nullptr) merged[i] = make_int2(te.token[i], __float_as_int(te.q[i]));
-    }
-    __syncwarp();
-    return;
-  }
+  for (int i = lane; i < k; i += 32)
+    if (te.token[i] >= 0) bits[te.token[i] / 32 % kNameWords] = 0;
+  __syncwarp();
+  return twice;
+}
+
+// Which entries are the first to name their token, and with `merged` the listed tokens, each once, with the sum of what its entries
+// have, by one warp.  `twice`: a token may be named more than once.
+__device__ __forceinline__ void mergeTeacher(Teacher& te, int k, bool twice, int2* merged) {
+  const int lane = threadIdx.x & 31;
   for (int i = lane; i < k; i += 32) {
     const int t = te.token[i];
-    float q = 0.f;
-    int before = k;
-    for (int j = 0; j < k; j += 4) {  // four at a time; behind the last of them is no token
-      const int4 o = *reinterpret_cast<const int4*>(&te.token[j]);
-      if (o.x == t) q += te.q[j], before = min(before, j);
-      if (o.y == t) q += te.q[j + 1], before = min(before, j + 1);
-      if (o.z == t) q += te.q[j + 2], before = min(before, j + 2);
-      if (o.w == t) q += te.q[j + 3], before = min(before, j + 3);
+    float q = te.q[i];
+    bool first = t >= 0;
+    if (twice) {
+      int before = k;
+      q = 0.f;
+      for (int j = 0; j < k; j += 4) {  // four at a time
+        const int4 o = *reinterpret_cast<const int4*>(&te.token[j]);
+        if (o.x == t) q += te.q[j], before = min(before, j);
+        if (o.y == t) q += te.q[j + 1], before = min(before, j + 1);
+        if (o.z == t) q += te.q[j + 2], before = min(before, j + 2);
+        if (o.w == t) q += te.q[j + 3], before = min(before, j + 3);
+      }
+      first = first && before == i;
     }
-    const bool first = t >= 0 && before == i;
     te.first[i] = first;
     if (merged != nullptr) merged[i] = make_int2(first ? t : -1, __float_as_int(q));
   }
   __syncwarp();
 }
 
-// Loss and what the backward needs, from the sums of the sweep, by one warp.  Kept: the maximum that the sweep takes
+// By one warp.
+template <bool kRest> __device__ __forceinline__ Listed listedOf(const Teacher& te, int k, float c) {
+  const int lane = threadIdx.x & 31;
+  Listed l = {te.log_terms, te.total, -INFINITY, 0.f, 0.f, -INFINITY, 0.f};
+  for (int i = lane; i < k; i += 32)
+    if (te.token[i] >= 0) l.ref = fmaxf(l.ref, te.logit[i]);
+  l.ref = warpMax(l.ref);
+  if (kRest) l.m = l.ref;
+  if (l.ref == -INFINITY) l.ref = 0.f;
+  for (int i = lane; i < k; i += 32) {
+    const float q = te.q[i], x = te.logit[i] - l.ref;
+    if (te.token[i] >= 0 && !(q == 0.f)) {
+      l.from_ref = fmaf(q, x, l.from_ref);
+      l.mass += q;
+    }
+    if (kRest && te.first[i]) l.s += exp2Of(x * c);
+  }
+  l.from_ref = warpSum(l.from_ref);
+  l.mass = warpSum(l.mass);
+  if (kRest) l.s = warpSum(l.s);
+  return l;
+}
+
+// Loss and what the backward needs, from that and the sums of the sweep, by one thread.  Kept: the maximum that the sweep takes
 // differences from and the factor of those exponentials, the same for the listed tokens; the last is -1 where the row does
 // not count.
 template <bool kRest>
-__device__ __forceinline__ void finishRow(const Teacher& te, int k, const Sums& acc, bool broken, float c, double inv_t, float* loss,
+__device__ __forceinline__ void finishRow(const Listed& l, const Sums& acc, bool broken, float c, double inv_t, float* loss,
                                           float4* stats) {
-  const int lane = threadIdx.x & 31;
   // All probabilities' maximum and sum; the sweep's are those of the rest.
-  float m = acc.m, s = acc.s;
+  float m = acc.m, s = acc.s, above = 1.f;
   if constexpr (kRest) {
-    for (int i = lane; i < k; i += 32)
-      if (te.first[i]) m = fmaxf(m, te.logit[i]);
-    m = warpMax(m);
-    float sum = 0.f;
-    for (int i = lane; i < k; i += 32)
-      if (te.first[i]) sum += exp2Of((te.logit[i] - m) * c);
-    s = acc.s * exp2Of((acc.m - m) * c) + warpSum(sum);
+    m = fmaxf(acc.m, l.m);
+    above = acc.s == 0.f ? 0.f : exp2Of((acc.m - m) * c);
+    s = acc.s * above + (l.s == 0.f ? 0.f : l.s * exp2Of((l.m - m) * c));
   }
-  // A divergence is a small difference of large logarithms: those are kept in 64 bits.
-  const double lse = (double)m * inv_t + log((double)s);
-  double sum = 0;
-  for (int i = lane; i < k; i += 32) {
-    const float q = te.q[i];
-    if (te.token[i] >= 0 && !(q == 0.f)) {
-      const double log_q = kRest ? (double)te.given[i] : (double)te.given[i] * inv_t - te.log_total;
-      sum += q * (log_q - ((double)te.logit[i] * inv_t - lse));
-    }
-  }
-  sum = warpSum(sum);
-  if (lane != 0) return;
-  const float nan = __int_as_float(0x7fffffff);  // NaN
+  const double lse = (double)m * inv_t + log((double)s), mass = l.mass;
+  double sum = l.log_terms - l.from_ref * inv_t;
+  if (!(mass == 0)) sum -= mass * (log((double)l.total) + (double)l.ref * inv_t - lse);
+  const float nan = __int_as_float(0x7fffffff);
   float4 st = make_float4(m, 1.f / s, m, 1.f / s);
   if constexpr (kRest) {
-    const double q_rest = 1.0 - te.mass < kLeastRest ? 0.0 : 1.0 - te.mass;  // NaN stays
+    const double q_rest = 1.0 - mass < kLeastRest ? 0.0 : 1.0 - mass;  // NaN stays
     if (!(q_rest == 0)) sum += q_rest * (log(q_rest) - ((double)acc.m * inv_t + log((double)acc.s) - lse));
-    const double all = te.mass + q_rest, p_rest = (double)(acc.s * exp2Of((acc.m - m) * c)) / s;
+    const double all = mass + q_rest, p_rest = (double)(acc.s * above) / s;
     const bool some = !(acc.s == 0.f);
     st = make_float4(some ? acc.m : 0.f, some ? (float)((all * p_rest - q_rest) / acc.s) : 0.f, m, (float)(all / s));
   }
@@ -210,21 +254,6 @@ __device__ __forceinline__ void finishRow(const Teacher& te, int k, const Sums& 
   *loss = broken ? nan : (float)sum;
 }
 
-// A row counts that has a listed token and, without the rest, one that the teacher gives some probability.
-template <bool kRest> struct Counts {
-  const int64_t* tokens;
-  const float* log_probs;
-  int k;
-  __device__ __forceinline__ bool entry(int64_t r, int i) const {
-    return tokens[r * k + i] >= 0 && (kRest || !(log_probs[r * k + i] == -INFINITY));
-  }
-  __device__ __forceinline__ bool operator()(int r) const {
-    bool some = entry(r, 0);
-    for (int i = 1; i < k && !some; ++i) some = entry(r, i);
-    return some;
-  }
-};
-
 __device__ __forceinline__ void skipRow(float* loss, float4* stats) {
   *loss = 0.f;
   *stats = make_float4(0.f, 0.f, 0.f, -1.f);
@@ -233,7 +262,7 @@ __device__ __forceinline__ void skipRow(float* loss, float4* stats) {
 // Few rows: one per cluster.
 template <typename T, bool kRest>
 __global__ void __launch_bounds__(kThreads, 4)
-distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRest> given, float c, double inv_t,
+distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given given, float c, double inv_t,
                            float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged) {
   namespace cg = cooperative_groups;
   __shared__ Teacher te;
@@ -252,7 +281,8 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRe
   if constexpr (kRest)
     for (int i = tid; i < Marks<T>::words(sl.v1 - sl.v0); i += kThreads) bits[i] = 0;
   bool some = false;
-  for (int i = tid; i < k; i += kThreads) some |= given.entry(r, i);
+  for (int i = tid; i < k; i += kThreads)
+    some |= given.tokens[r * k + i] >= 0 && (kRest || !(given.log_probs[r * k + i] == -INFINITY));
   if (!__syncthreads_or(some)) {
     if (rank == 0 && tid == 0) skipRow(loss + r, stats + r);
     return;
@@ -268,11 +298,11 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRe
     }
     __syncthreads();
   }
-  bool outside = false;
+  Listed l = {};
   if (rank == 0 && tid < 32) {
-    outside = loadTeacher(te, given.tokens, given.log_probs, k, r, x.vocab);
-    loadLogits(te, k, row);
-    teacherOf<kRest>(te, k, (float)inv_t, true, merged != nullptr ? merged + r * k : nullptr);
+    loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
+    mergeTeacher(te, k, true, merged != nullptr ? merged + r * k : nullptr);
+    l = listedOf<kRest>(te, k, c);
   }
   Sums acc;
   if constexpr (kRest) {
@@ -297,27 +327,34 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRe
     else
       acc = blockAgain<T, false>(row, x.vocab, c, scratch, LeaveNone());
   }
-  if (tid < 32) finishRow<kRest>(te, k, acc, outside, c, inv_t, loss + r, stats + r);
+  if (tid == 0) finishRow<kRest>(l, acc, te.outside, c, inv_t, loss + r, stats + r);
 }
 
-// Many rows: the blocks stay.  With the rest a finishing warp marks the listed tokens of its next row while the rows before
-// it are swept, and takes the marks away when it is done.
-constexpr int kFinishers = 64, kFinishWarps = kFinishers / 32;
-constexpr int kUnfinished = kFinishWarps;
-constexpr int kNameWords = 1024;
+// Many rows: the blocks stay.  With the rest the fetching warp marks the listed tokens of a row while the row before it is
+// swept, in place of those of the row before that.
+// A row that needs no more than finishRow(), which is done for 32 of them at once.
+struct Pending {
+  Listed listed;
+  Sums sums;
+  int row;
+  bool outside;
+};
 struct DistillRows {
   Ring ring;
-  HandOver<kUnfinished> hand;
-  Teacher teacher[kFinishWarps];
-  alignas(16) unsigned bits[1];  // words for each finishing warp: marks of a row's listed tokens
+  HandOver hand;
+  Teacher teacher[kSlots];
+  unsigned loose[kSlots];  // the listed columns outside the vectors
+  Pending pending[32];
+  alignas(16) unsigned bits[1];  // with the rest twice, else once, as many words as the kernel is told
 };
 template <typename T> struct RestRowsHook : RestHook {
-  HandOver<kUnfinished>* hand;
   const unsigned* all;
-  int words_a_row;
-  __device__ __forceinline__ void begin(int buffer, unsigned parity) {
-    hand->wait(&hand->ready[buffer], parity);
-    bits = all + buffer * words_a_row;
+  HandOver* hand;
+  int words_a_row, turn = 1;
+  __device__ __forceinline__ void begin(const Place& at) {
+    hand->wait(&hand->marked[at.slot], at.parity);
+    turn ^= 1;
+    bits = all + turn * words_a_row;
   }
   __device__ __forceinline__ void end() {}
   __device__ __forceinline__ void arrived(uint4* place, int b) {
@@ -330,77 +367,114 @@ template <typename T> struct RestRowsHook : RestHook {
   __device__ __forceinline__ float batch(uint4 (&now)[kBatch], bool, int, const Slice<T>&) { return batchMax<T>(now); }
 };
 template <typename T, bool kRest>
-__global__ void __launch_bounds__(kThreads + kFinishers, 3)
-distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Counts<kRest> counts, float c, double inv_t,
-                         float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged, int words) {
+__global__ void __launch_bounds__(kRowThreads, 3)
+distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Given given, float c, double inv_t,
+                         float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged, int words, int rows_a_block) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   DistillRows& shared = *reinterpret_cast<DistillRows*>(dynamic);
-  HandOver<kUnfinished>& hand = shared.hand;
+  HandOver& hand = shared.hand;
   if (threadIdx.x == 0) hand.init();
-  for (int i = threadIdx.x; i < words * kUnfinished; i += kThreads + kFinishers)
-    shared.bits[i] = 0;
+  for (int i = threadIdx.x; i < words * (kRest ? 2 : 1); i += kRowThreads) shared.bits[i] = 0;
   __syncthreads();
   if (threadIdx.x < kThreads) {
     if constexpr (kRest) {
       RestRowsHook<T> hook;
-      hook.hand = &hand;
       hook.all = shared.bits;
+      hook.hand = &hand;
       hook.words_a_row = words;
-      sweepRows<T, false>(logits, x, counts, c, shared.ring, hand, hook);
+      sweepRows<T, false>(logits, x, c, shared.ring, hand, hook);
     } else {
       NoHook none;
-      sweepRows<T, false>(logits, x, counts, c, shared.ring, hand, none);
+      sweepRows<T, false>(logits, x, c, shared.ring, hand, none);
     }
     return;
   }
-  const int which = (int)(threadIdx.x - kThreads) / 32, lane = threadIdx.x & 31, k = counts.k;
-  Teacher& te = shared.teacher[which];
-  const auto finish = [&](int64_t r, int buffer, unsigned parity) {
+  const int lane = threadIdx.x & 31, k = given.k;
+  if (threadIdx.x < kThreads + 32) {
+    Place before;  // the row before the last
+    int fetched = 0, marked = -1, marked_before = -1;  // the rows whose listed tokens are marked
+    fetchRows(
+        [](int) { return true; }, x.rows, rows_a_block, hand, [&](int r) { skipRow(loss + r, stats + r); },
+        [&](int r, const Place& at) {
+          if (!countsAtAll<kRest>(given, r)) return false;
+          const float nan = __int_as_float(0x7fffffff);
+          if (lane == 0) loss[r] = nan, stats[r] = make_float4(nan, nan, nan, nan);  // stays if nobody comes to finish the row
+          // The marks are waited for, so what can be done before the row is handed on is.
+          if (kRest) loadTeacher<T, kRest>(shared.teacher[at.slot], given, r, rowOf(x, logits, r), x.vocab, (float)inv_t);
+          return true;
+        },
+        [&](int r, const Place& at) {
+          Teacher& te = shared.teacher[at.slot];
+          const T* row = rowOf(x, logits, r);
+          if (!kRest) loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
+          bool twice = false;
+          {
+            if constexpr (kRest) {
+              unsigned* bits = shared.bits + (fetched & 1) * words;
+              if (fetched >= 2) {  // swept: its marks go
+                hand.wait(&hand.full[before.slot], before.parity);
+                const Slice<T> sl(rowOf(x, logits, marked_before), x.vocab, 0, 1);
+                const Teacher& old = shared.teacher[before.slot];
+                for (int i = lane; i < k; i += 32)
+                  if (old.token[i] >= 0 && !Marks<T>::loose(sl, old.token[i])) bits[Marks<T>::place(sl, old.token[i]) >> 5] = 0;
+                before.next();
+                __syncwarp();
+              }
+              marked_before = marked;
+              marked = r;
+              const Slice<T> sl(row, x.vocab, 0, 1);
+              unsigned loose = 0;
+              for (int i = lane; i < k; i += 32) {
+                const int t = te.token[i];
+                if (t < 0) continue;
+                if (Marks<T>::loose(sl, t))
+                  loose |= Marks<T>::looseBit(sl, t), twice = true;  // perhaps: there are few
+                else
+                  twice |= setBit(bits, Marks<T>::place(sl, t));
+              }
+              loose = __reduce_or_sync(kAll, loose);
+              if (lane == 0) {
+                shared.loose[at.slot] = loose;
+                barrierArrive(&hand.marked[at.slot]);
+              }
+              ++fetched;
+            } else if (merged != nullptr) {
+              twice = namedTwice(te, k, shared.bits);
+            }
+          }
+          if (kRest || merged != nullptr)
+            mergeTeacher(te, k, kRest ? __any_sync(kAll, twice) : twice, merged != nullptr ? merged + (int64_t)r * k : nullptr);
+        });
+    return;
+  }
+  int pending = 0;
+  auto flush = [&] {
+    __syncwarp();
+    if (lane < pending) {
+      const Pending& p = shared.pending[lane];
+      finishRow<kRest>(p.listed, p.sums, p.outside, c, inv_t, loss + p.row, stats + p.row);
+    }
+    __syncwarp();
+    pending = 0;
+  };
+  finishRows(hand, [&](int r, const Place& at) {
     const T* row = rowOf(x, logits, r);
     const Slice<T> sl(row, x.vocab, 0, 1);
-    const bool outside = loadTeacher(te, counts.tokens, counts.log_probs, k, r, x.vocab);
-    unsigned left_out = 0;
-    unsigned* bits = shared.bits + buffer * words;
-    bool twice = false;
-    if constexpr (kRest) {
-      for (int i = lane; i < k; i += 32) {
-        const int t = te.token[i];
-        if (t < 0) continue;
-        if (Marks<T>::loose(sl, t))
-          left_out |= Marks<T>::looseBit(sl, t), twice = true;  // perhaps: there are few
-        else
-          twice |= setBit(bits, Marks<T>::place(sl, t));
-      }
-      left_out = __reduce_or_sync(kAll, left_out);
-      if (lane == 0) barrierArrive(&hand.ready[buffer]);
-    } else {  // a token's bit is that of its number's end: two that differ may share it, which costs time alone
-      for (int i = lane; i < k; i += 32)
-        if (te.token[i] >= 0) twice |= setBit(bits, te.token[i] % (32 * kNameWords));
-      __syncwarp();
-      for (int i = lane; i < k; i += 32)
-        if (te.token[i] >= 0) clearBit(bits, te.token[i] % (32 * kNameWords));
-    }
-    teacherOf<kRest>(te, k, (float)inv_t, __any_sync(kAll, twice), merged != nullptr ? merged + r * k : nullptr);
-    hand.wait(&hand.full[buffer], parity);
-    loadLogits(te, k, row);  // swept not long ago: from L2
-    Sums acc = hand.template take<T, false>(buffer, sl, c, left_out);
-    if constexpr (kRest)
-      for (int i = lane; i < k; i += 32)
-        if (te.token[i] >= 0 && !Marks<T>::loose(sl, te.token[i])) clearBit(bits, Marks<T>::place(sl, te.token[i]));
-    __syncwarp();
-    if (lane == 0) barrierArrive(&hand.empty[buffer]);
+    const Teacher& te = shared.teacher[at.slot];
+    if (!hand.wait(&hand.prepared[at.slot], at.parity)) return;
+    const Listed l = listedOf<kRest>(te, k, c);
+    if (!hand.wait(&hand.full[at.slot], at.parity)) return;
+    Sums acc = hand.template take<T, false>(at.slot, sl, c, kRest ? shared.loose[at.slot] : 0);
     if (!acc.settle<false>(c)) {
       if constexpr (kRest)
         acc = warpAgain<T, false>(row, x.vocab, c, LeaveListed{&te, k});
       else
         acc = warpAgain<T, false>(row, x.vocab, c, LeaveNone());
     }
-    finishRow<kRest>(te, k, acc, outside || hand.gaveUp(), c, inv_t, loss + r, stats + r);
-    __syncwarp();
-  };
-  finishRows<kUnfinished>(counts, x.rows, which, kFinishWarps, finish, [&](int64_t r) {
-    if (which == 0) skipRow(loss + r, stats + r);
+    if (lane == 0) shared.pending[pending] = {l, acc, r, te.outside};
+    if (++pending == 32) flush();
   });
+  flush();
 }
 
 __global__ void __launch_bounds__(1024)
@@ -493,13 +567,15 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArg
                       int sm_count, cudaStream_t stream) {
   const float c = (float)(1.4426950408889634 / a.temperature);
   const double inv_t = 1.0 / a.temperature;
-  const Counts<kRest> counts{a.tokens, a.log_probs, a.k};
+  const Given given{a.tokens, a.log_probs, a.k};
   const int words = kRest ? Marks<T>::words(x.vocab / Vec<T>::kElems) : kNameWords;
-  const size_t stay = sizeof(DistillRows) + kUnfinished * (size_t)words * 4;
-  // Two blocks of the form that stays have to fit on a multiprocessor, with up to 70,000 tokens three do.
-  if (manyRows(x.rows, sm_count) && stay <= 112 * 1024)
-    return launchResident(distillation_rows_kernel<T, kRest>, x.rows, kThreads + kFinishers, stay <= 75 * 1024 ? 3 : 2, stay, sm_count,
-                          stream, logits, x, counts, c, inv_t, loss, stats, merged, words);
+  const size_t stay = sizeof(DistillRows) + (kRest ? 2 : 1) * (size_t)words * 4;
+  // Two blocks of the form that stays have to fit on a multiprocessor; up to 65536 tokens of 16 bits three do.
+  if (manyRows(x.rows, sm_count) && stay <= 112 * 1024) {
+    const int rows_a_block = rowsABlock(x, sizeof(T));
+    return launchRows(distillation_rows_kernel<T, kRest>, x.rows, rows_a_block, stay, stream, logits, x, given, c, inv_t, loss, stats,
+                      merged, words, rows_a_block);
+  }
   const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
   const size_t shared = kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) * 4 : 0;
   if (shared > 32 * 1024) {
@@ -507,7 +583,7 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArg
                                                (int)shared);
     if (e != cudaSuccess) return e;
   }
-  return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, shared, stream, logits, x, counts, c, inv_t, loss,
+  return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, shared, stream, logits, x, given, c, inv_t, loss,
                       stats, merged);
 }
 

@@ -282,7 +282,7 @@ struct Exponent {
 
 // What a kernel does with a batch, that from vector i on, before it is summed; returns its largest value.
 struct NoHook {
-  __device__ __forceinline__ void begin(int, unsigned) {}
+  template <typename P> __device__ __forceinline__ void begin(const P&) {}
   __device__ __forceinline__ void end() {}
   __device__ __forceinline__ void arrived(uint4*, int) {}
   template <typename T> __device__ __forceinline__ float batch(uint4 (&now)[kBatch], bool, int, const Slice<T>&) {
@@ -442,15 +442,18 @@ cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, si
 
 // ---- many rows -----------------------------------------------------------------
 // With a block per row the memory idles while a block starts and while it finishes its row, three to four
-// microseconds of the ten that the row itself takes (8192 x 51200 bf16: 144 us for the log probabilities, 4.6 to 5.8 TB/s).
-// So where there are many rows the blocks stay and take row after row in three roles:
+// microseconds of the ten that the row itself takes.  So where there are many rows the blocks stay and take row after row
+// in three roles:
+//  - one warp fetches rows: it asks the hardware for a block that has not started yet and takes over that block's rows,
+//    so that blocks which get more of the memory's bandwidth do more of them; it prepares what needs no look at the logits;
 //  - eight warps sweep: every thread copies its own vectors to shared memory, kDepth - 1 batches ahead and
 //    across the ends of rows, and waits for its own copies alone;
-//  - they hand each row's sums over and go on without waiting;
-//  - the other warps finish rows: what needs no sums they do while the row is swept.
+//  - one warp finishes rows while the next ones are swept.
 constexpr int kManyRows = 4;  // for each multiprocessor
 constexpr int kDepth = 3;
-constexpr int kSpins = 1 << 20;  // tries, each of which the hardware lets sleep; then the wait is given up
+constexpr int kRowThreads = kThreads + 64;  // sweep, then the warp that fetches, then the one that finishes
+constexpr int kSlots = 3;                   // rows between being fetched and being finished
+constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait is given up
 
 __device__ __forceinline__ uint32_t sharedAddress(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrierInit(uint64_t* bar, int arrivals) {
@@ -459,17 +462,26 @@ __device__ __forceinline__ void barrierInit(uint64_t* bar, int arrivals) {
 __device__ __forceinline__ void barrierArrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sharedAddress(bar)) : "memory");
 }
+__device__ __forceinline__ bool barrierTry(uint64_t* bar, unsigned parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(sharedAddress(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ uint64_t nanoseconds() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
 __device__ __forceinline__ bool barrierWait(uint64_t* bar, unsigned parity) {
-  for (int i = 0; i < kSpins; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(sharedAddress(bar)), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return false;
+  if (barrierTry(bar, parity)) return true;
+  const uint64_t start = nanoseconds();
+  while (!barrierTry(bar, parity))
+    if (nanoseconds() - start > kPatience) return false;
+  return true;
 }
 __device__ __forceinline__ void copyAhead(uint4* to, const uint4* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sharedAddress(to)), "l"(from) : "memory");
@@ -477,115 +489,179 @@ __device__ __forceinline__ void copyAhead(uint4* to, const uint4* from) {
 __device__ __forceinline__ void commitCopies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kLeft> __device__ __forceinline__ void waitCopies() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
 
-// The rows of this block that count, in order, as every warp finds them for itself: a lane looks at one of the next 32.
-template <class Counts> struct RowWalk {
-  const Counts& counts;
-  const unsigned rows;
-  unsigned base;      // the row of lane 0
-  unsigned mask = 0;  // of those not yet taken
-  int row = -1;       // the current one; -1: none left
-  __device__ __forceinline__ RowWalk(const Counts& counts_, int64_t rows_)
-      : counts(counts_), rows((unsigned)rows_), base(blockIdx.x - 32 * gridDim.x) {}
-  template <class Skip> __device__ __forceinline__ void next(Skip&& skip) {
-    while (mask == 0) {
-      base += 32 * gridDim.x;
-      if (base >= rows) {
-        base -= 32 * gridDim.x;
-        row = -1;
-        return;
-      }
-      const unsigned mine = base + (threadIdx.x & 31) * gridDim.x;
-      const bool some = mine < rows, yes = some && counts((int)mine);
-      if (some && !yes) skip((int)mine);
-      mask = __ballot_sync(kAll, yes);
-    }
-    row = (int)(base + (__ffs(mask) - 1) * gridDim.x);
-    mask &= mask - 1;
-  }
+// A place in the sequence of slots.
+struct Place {
+  int slot = 0;
+  unsigned parity = 0;
   __device__ __forceinline__ void next() {
-    next([](int) {});
+    if (++slot == kSlots) slot = 0, parity ^= 1;
   }
 };
 
-// What the sweeping warps hand over, for as many rows as may be unfinished at once.
-template <int kRows> struct HandOver {
-  // The row's listed tokens are marked; its sums are there; the buffer is free for another row.
-  uint64_t ready[kRows], full[kRows], empty[kRows];
-  Sums sums[kRows][kWarps];
+// The rows that a block has taken.  Whoever gives up a wait has the block stop; what it has taken and not finished is NaN, which the
+// fetching warp writes before it hands a row on.
+struct HandOver {
+  alignas(16) uint4 answer;
+  uint64_t answered;
+  // The row is there; what its sweep needs is (the hook waits for that); what its finish needs is; its sums are; the slot is free.
+  uint64_t ready[kSlots], marked[kSlots], prepared[kSlots], full[kSlots], empty[kSlots];
+  Sums sums[kSlots][kWarps];
+  int row[kSlots];  // -1: there are no more
   int failed;
   // By one thread, before a barrier of the block.
   __device__ __forceinline__ void init() {
-    for (int i = 0; i < kRows; ++i) {
+    barrierInit(&answered, 1);
+    for (int i = 0; i < kSlots; ++i) {
       barrierInit(&ready[i], 1);
+      barrierInit(&marked[i], 1);
+      barrierInit(&prepared[i], 1);
       barrierInit(&full[i], kWarps);
       barrierInit(&empty[i], 1);
     }
     failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // All lanes of a warp.  Once a wait was given up nobody waits any more, and the block's rows become NaN.
-  __device__ __forceinline__ void wait(uint64_t* bar, unsigned parity) {
+  __device__ __forceinline__ bool gaveUp() const { return *static_cast<const volatile int*>(&failed) != 0; }
+  // All lanes of a warp; false once somebody gave up.
+  __device__ __forceinline__ bool wait(uint64_t* bar, unsigned parity) {
     if (!gaveUp() && !barrierWait(bar, parity)) *static_cast<volatile int*>(&failed) = 1;
     __syncwarp();
+    return !gaveUp();
+  }
+  __device__ __forceinline__ int rowAt(const Place& p) { return wait(&ready[p.slot], p.parity) ? row[p.slot] : -1; }
+  // By one thread: asks for the block that would start next; the one before must have been answered with one.
+  __device__ __forceinline__ void ask() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], 16;" ::"r"(sharedAddress(&answered)) : "memory");
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     sharedAddress(&answer)),
+                 "r"(sharedAddress(&answered))
+                 : "memory");
+  }
+  // By a warp: the number of the block that will not start, or -1 if all have.
+  __device__ __forceinline__ int answerOf(unsigned parity) {
+    if (!wait(&answered, parity)) return -1;
+    int block;
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .b128 r;\nld.shared.b128 r, [%2];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\nselp.u32 %1, 1, 0, p;\nmov.u32 %0, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n}"
+        : "=r"(block), "=r"(ok)
+        : "r"(sharedAddress(&answer))
+        : "memory");
+    __syncwarp();
+    return ok ? block : -1;
   }
   // The row's sums in every lane of a warp; the columns outside the vectors are added here.
   // `left_out`: a bit for each of those that is not to be.
   template <typename T, bool kEntropy>
-  __device__ __forceinline__ Sums take(int buffer, const Slice<T>& sl, float c, unsigned left_out) const {
+  __device__ __forceinline__ Sums take(int slot, const Slice<T>& sl, float c, unsigned left_out) const {
     const int lane = threadIdx.x & 31;
-    Sums acc = lane < kWarps ? sums[buffer][lane] : Sums::none(c);
+    Sums acc = lane < kWarps ? sums[slot][lane] : Sums::none(c);
     const int col = lane < 2 * Vec<T>::kElems && !(left_out >> lane & 1u) ? sl.looseCol(lane) : -1;
     if (col >= 0) acc.add<kEntropy>(toFloat(sl.row[col]), c);
     return warpSums<kEntropy>(acc, c);
   }
-  __device__ __forceinline__ bool gaveUp() const { return *static_cast<const volatile int*>(&failed) != 0; }
 };
 
 using Ring = uint4[kDepth][kBatch][kThreads];
 
+// How many rows a block of the grid stands for: as many as make up 64 KB, so that asking for them does not cost more than they do.
+inline int rowsABlock(const LogitRows& x, int elem_size) {
+  const int64_t n = (65536 + (int64_t)x.vocab * elem_size - 1) / ((int64_t)x.vocab * elem_size);
+  return n < 32 ? (int)n : 32;
+}
+
+// The fetching warp's part.  `counts(r)`, by one lane, says that a row does not count as far as that is seen at once, else skip(r), by
+// one lane too.  prepare(r, place), by all, says for the others whether they do; mark(r, place) comes once the row's copies may begin.
+// Copies run kDepth - 1 batches ahead, so as many rows: nothing that a row's copies wait for may itself wait for one of the
+// kSlots - 1 rows before it.
+static_assert(kSlots >= kDepth, "a row's copies begin while the row kDepth - 1 before it is swept");
+template <class Counts, class Skip, class Prepare, class Mark>
+__device__ __forceinline__ void fetchRows(Counts&& counts, int64_t rows, int rows_a_block, HandOver& out, Skip&& skip,
+                                          Prepare&& prepare, Mark&& mark) {
+  const int lane = threadIdx.x & 31;
+  Place place;
+  unsigned parity = 0;
+  for (int block = blockIdx.x; block >= 0; parity ^= 1) {
+    if (lane == 0) out.ask();
+    const int64_t first = (int64_t)block * rows_a_block, mine = first + lane;
+    const bool some = lane < rows_a_block && mine < rows, yes = some && counts((int)mine);
+    if (some && !yes) skip((int)mine);
+    for (unsigned mask = __ballot_sync(kAll, yes); mask != 0; mask &= mask - 1) {
+      const int r = (int)first + __ffs(mask) - 1;
+      if (!out.wait(&out.empty[place.slot], place.parity ^ 1)) {
+        barrierWait(&out.answered, parity);  // the answer is on its way to this block's memory
+        return;
+      }
+      if (!prepare(r, place)) {
+        if (lane == 0) skip(r);
+        continue;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        out.row[place.slot] = r;
+        barrierArrive(&out.ready[place.slot]);
+      }
+      mark(r, place);
+      __syncwarp();
+      if (lane == 0) barrierArrive(&out.prepared[place.slot]);
+      place.next();
+    }
+    block = out.answerOf(parity);
+  }
+  if (!out.wait(&out.empty[place.slot], place.parity ^ 1)) return;
+  if (lane == 0) {
+    out.row[place.slot] = -1;
+    barrierArrive(&out.ready[place.slot]);
+  }
+}
+
 // The sweeping warps' part, threads 0 to kThreads - 1.  The hook sees a thread's part of batch b of a row in shared memory
 // before it is read.
-template <typename T, bool kEntropy, int kRows, class Hook, class Counts>
-__device__ __forceinline__ void sweepRows(const T* logits, const LogitRows& x, const Counts& counts, float c, Ring& ring,
-                                          HandOver<kRows>& out, Hook& hook) {
+template <typename T, bool kEntropy, class Hook>
+__device__ __forceinline__ void sweepRows(const T* logits, const LogitRows& x, float c, Ring& ring, HandOver& out, Hook& hook) {
   constexpr int U = kBatch;
   constexpr uint32_t w = Vec<T>::kMinusInf;
   const int tid = threadIdx.x;
-  RowWalk<Counts> ahead(counts, x.rows), at(counts, x.rows);  // the row that is copied and the one that is summed
+  Place ahead, at;              // the row that is copied and the one that is summed
   const uint4* from = nullptr;  // of the row that is copied: this thread's next vector,
-  int whole = 0, left = 0;      // the batches that all threads have, and the vectors from this thread's on behind those; < 0: no row
+  int whole = 0, left = -1;     // the batches that all threads have, and the vectors behind those; < 0: the row is through
+  bool more = true;
   auto open = [&] {
+    const int r = out.rowAt(ahead);
+    more = r >= 0;
+    if (!more) return;
     ahead.next();
-    left = -kThreads;
-    if (ahead.row < 0) return;
-    const T* row = rowOf(x, logits, ahead.row);
+    const T* row = rowOf(x, logits, r);
     const RowParts<T> parts(row, x.vocab);
     from = reinterpret_cast<const uint4*>(row + parts.head) + tid;
     whole = parts.nvec / (U * kThreads);
     left = parts.nvec - whole * (U * kThreads);
+    if (whole > 0 && left == 0) left = -1;
   };
   auto issue = [&](int slot) {
+    if (whole == 0 && left < 0 && more) open();
     uint4* to = &ring[slot][0][tid];
     if (__any_sync(kAll, whole > 0)) {
 #pragma unroll
       for (int u = 0; u < U; ++u) copyAhead(to + u * kThreads, from + u * kThreads);
       from += U * kThreads;
-      if (--whole == 0 && left == 0) open();
+      --whole;
     } else if (left >= 0) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (tid + u * kThreads < left) copyAhead(to + u * kThreads, from + u * kThreads);
-      open();
+      left = -1;
     }
     commitCopies();
   };
-  open();
 #pragma unroll
   for (int d = 0; d < kDepth - 1; ++d) issue(d);
-  int slot = 0, buffer = 0;
-  unsigned parity = 0;
+  int slot = 0;
   uint4 now[U];
-  auto take = [&](int b) {  // the row's batch b, whose turn it is; the place of the one before it, whose values have been used, is filled again
+  auto take = [&](int b) {  // the row's batch b; the place of the one before it, whose values have been used, is filled again
     waitCopies<kDepth - 2>();
     uint4* place = &ring[slot][0][tid];
     hook.arrived(place, b);
@@ -594,10 +670,11 @@ __device__ __forceinline__ void sweepRows(const T* logits, const LogitRows& x, c
     issue(slot == 0 ? kDepth - 1 : slot - 1);
     slot = slot + 1 == kDepth ? 0 : slot + 1;
   };
-  for (at.next(); at.row >= 0; at.next()) {
-    const Slice<T> sl(rowOf(x, logits, at.row), x.vocab, 0, 1);
-    out.wait(&out.empty[buffer], parity ^ 1);
-    hook.begin(buffer, parity);
+  for (;; at.next()) {
+    const int r = out.rowAt(at);
+    if (r < 0) break;
+    const Slice<T> sl(rowOf(x, logits, r), x.vocab, 0, 1);
+    hook.begin(at);
     ThreadSums mine(c);
     const int batches = sl.v1 / (U * kThreads), rest = sl.v1 - batches * (U * kThreads);
     for (int b = 0; b < batches; ++b) {
@@ -615,37 +692,29 @@ __device__ __forceinline__ void sweepRows(const T* logits, const LogitRows& x, c
     hook.end();
     const Sums acc = warpSums<kEntropy>(mine.sums(), c);
     if ((tid & 31) == 0) {
-      out.sums[buffer][tid >> 5] = acc;
-      barrierArrive(&out.full[buffer]);
+      out.sums[at.slot][tid >> 5] = acc;
+      barrierArrive(&out.full[at.slot]);
     }
-    if (++buffer == kRows) buffer = 0, parity ^= 1;
   }
   waitCopies<0>();
 }
 
-// A finishing warp's or group's part: finish(row, buffer, parity) for those of the rows that count whose number is `which`
-// modulo `each`, skip(row) by single lanes for those that do not.
-template <int kRows, class Counts, class Finish, class Skip>
-__device__ __forceinline__ void finishRows(const Counts& counts, int64_t rows, int which, int each, Finish&& finish, Skip&& skip) {
-  RowWalk<Counts> at(counts, rows);
-  int buffer = 0, turn = 0;
-  unsigned parity = 0;
-  for (at.next(skip); at.row >= 0; at.next(skip)) {
-    if (turn == which) finish(at.row, buffer, parity);
-    if (++turn == each) turn = 0;
-    if (++buffer == kRows) buffer = 0, parity ^= 1;
+// The finishing warp's part: finish(r, place), which waits for the row's sums.
+template <class Finish> __device__ __forceinline__ void finishRows(HandOver& out, Finish&& finish) {
+  for (Place at;; at.next()) {
+    const int r = out.rowAt(at);
+    if (r < 0) return;
+    finish(r, at);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) barrierArrive(&out.empty[at.slot]);
   }
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launchResident(void (*kernel)(Params...), int64_t rows, int threads, int blocks_per_sm, size_t shared,
-                           int sm_count, cudaStream_t stream, Args... args) {
+cudaError_t launchRows(void (*kernel)(Params...), int64_t rows, int rows_a_block, size_t shared, cudaStream_t stream, Args... args) {
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
   if (e != cudaSuccess) return e;
-  // Those that stay, or one for six rows: blocks do not get equal shares of the memory's bandwidth, and the hardware
-  // hands out the later ones to whoever is done.
-  const int64_t stay = (int64_t)blocks_per_sm * sm_count, blocks = rows / 6 > stay ? rows / 6 : stay;
-  kernel<<<(unsigned)(rows < blocks ? rows : blocks), threads, shared, stream>>>(Params(args)...);
+  kernel<<<(unsigned)((rows + rows_a_block - 1) / rows_a_block), kRowThreads, shared, stream>>>(Params(args)...);
   noteLocalLaunch();
   return cudaGetLastError();
 }

@@ -329,6 +329,13 @@ struct Outputs {
       top_tokens[r * k + i] = -1;
     }
   }
+  // By one thread: what stays if nobody comes to finish the row.
+  __device__ __forceinline__ void broken(int64_t r) const {
+    const float nan = __int_as_float(0x7fffffff);
+    if (log_probs != nullptr) log_probs[r] = nan;
+    if (entropy != nullptr) entropy[r] = nan;
+    if (stats != nullptr) stats[r] = make_float2(0.f, nan);
+  }
   // By one thread; `logit` is the token's.
   template <bool kEntropy>
   __device__ __forceinline__ void values(int64_t r, const Sums& acc, bool known, float logit, float c, float inv_t) const {
@@ -402,43 +409,44 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
 }
 
 // Many rows: the blocks stay.
-constexpr int kFinishers = 64, kUnfinished = 4;
 struct Rows {
   Ring ring;
-  HandOver<kUnfinished> hand;
+  HandOver hand;
 };
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(kThreads + kFinishers, 3)
-token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t) {
+__global__ void __launch_bounds__(kRowThreads, 3)
+token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t, int rows_a_block) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   Rows& shared = *reinterpret_cast<Rows*>(dynamic);
-  HandOver<kUnfinished>& hand = shared.hand;
+  HandOver& hand = shared.hand;
   if (threadIdx.x == 0) hand.init();
   __syncthreads();
   const int64_t* tokens = out.tokens;
-  const auto counts = [tokens](int r) { return tokens == nullptr || tokens[r] >= 0; };
   if (threadIdx.x < kThreads) {
     NoHook none;
-    sweepRows<T, kEntropy>(logits, x, counts, c, shared.ring, hand, none);
+    sweepRows<T, kEntropy>(logits, x, c, shared.ring, hand, none);
     return;
   }
-  const int which = (int)(threadIdx.x - kThreads) / 32, lane = threadIdx.x & 31;
-  const auto finish = [&](int64_t r, int buffer, unsigned parity) {
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < kThreads + 32) {
+    fetchRows(
+        [&](int r) { return tokens == nullptr || tokens[r] >= 0; }, x.rows, rows_a_block, hand, [&](int r) { out.skipped(r); },
+        [&](int r, const Place&) {
+          if (lane == 0) out.broken(r);
+          return true;
+        },
+        [](int, const Place&) {});
+    return;
+  }
+  finishRows(hand, [&](int r, const Place& at) {
     const Slice<T> sl(rowOf(x, logits, r), x.vocab, 0, 1);
     const int64_t t = tokens != nullptr ? tokens[r] : 0;
     const bool known = t < x.vocab;
     const float logit = known ? toFloat(sl.row[t]) : 0.f;
-    hand.wait(&hand.full[buffer], parity);
-    Sums acc = hand.template take<T, kEntropy>(buffer, sl, c, 0);
-    __syncwarp();
-    if (lane == 0) barrierArrive(&hand.empty[buffer]);
+    if (!hand.wait(&hand.full[at.slot], at.parity)) return;
+    Sums acc = hand.template take<T, kEntropy>(at.slot, sl, c, 0);
     if (!acc.template settle<kEntropy>(c)) acc = warpAgain<T, kEntropy>(sl.row, x.vocab, c, LeaveNone());
-    if (hand.gaveUp()) acc.s = __int_as_float(0x7fffffff);
-    if (lane != 0) return;
-    out.values<kEntropy>(r, acc, known, logit, c, inv_t);
-  };
-  finishRows<kUnfinished>(counts, x.rows, which, kFinishers / 32, finish, [&](int64_t r) {
-    if (which == 0) out.skipped(r);
+    if (lane == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
   });
 }
 
@@ -512,9 +520,11 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restr
 template <typename T, bool kEntropy>
 cudaError_t forwardOf(const T* logits, const LogitRows& x, const Outputs& out, double temperature, int sm_count, cudaStream_t stream) {
   const float inv_t = (float)(1.0 / temperature), c = (float)(1.4426950408889634 / temperature);
-  if (out.k == 0 && manyRows(x.rows, sm_count))
-    return launchResident(token_log_probs_rows_kernel<T, kEntropy>, x.rows, kThreads + kFinishers, 3, sizeof(Rows), sm_count,
-                          stream, logits, x, out, c, inv_t);
+  if (out.k == 0 && manyRows(x.rows, sm_count)) {
+    const int rows_a_block = rowsABlock(x, sizeof(T));
+    return launchRows(token_log_probs_rows_kernel<T, kEntropy>, x.rows, rows_a_block, sizeof(Rows), stream, logits, x, out, c, inv_t,
+                      rows_a_block);
+  }
   const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
   if (out.k > 0)
     return launchSlices(token_log_probs_slices_kernel<T, kEntropy, true>, x.rows, slices,

@@ -21,16 +21,16 @@ using torch::autograd::variable_list;
 int multiprocessors() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 
 void checkLogits(const at::Tensor& logits) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() >= 1, "logits must be a CUDA tensor of at least one dimension");
-  TORCH_CHECK(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 ||
-                  logits.scalar_type() == at::kHalf,
-              "logits must be fp32, bf16 or fp16");
-  TORCH_CHECK(logits.size(-1) > 0 && logits.size(-1) <= INT32_MAX - 64, "the vocabulary must not be empty");
-  TORCH_CHECK(logits.numel() / logits.size(-1) <= INT32_MAX, "too many rows");
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1, "logits must be a CUDA tensor of at least one dimension");
+  TORCH_CHECK_VALUE(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 ||
+                        logits.scalar_type() == at::kHalf,
+                    "logits must be fp32, bf16 or fp16");
+  TORCH_CHECK_VALUE(logits.size(-1) > 0 && logits.size(-1) <= INT32_MAX - 64, "the vocabulary must not be empty");
+  TORCH_CHECK_VALUE(logits.numel() / logits.size(-1) <= INT32_MAX, "too many rows");
 }
 
 void checkTemperature(double t) {
-  TORCH_CHECK(t >= 1e-30 && t <= 1e30, "the temperature must be positive and finite, from 1e-30 to 1e30");
+  TORCH_CHECK_VALUE(t >= 1e-30 && t <= 1e30, "temperature must be positive and finite, from 1e-30 to 1e30, not ", t);
 }
 
 // Logits whose rows the kernels can walk, and how: the leading dimensions as two levels of strides, the last
@@ -107,10 +107,12 @@ std::tuple<at::Tensor, int64_t> perRow(const at::Tensor& g) {
   return std::make_tuple(t.contiguous(), 1);
 }
 
+// int64, contiguous, from integers of that shape on the logits' device.
 at::Tensor checkTokens(const at::Tensor& tokens, const at::Tensor& logits, at::IntArrayRef sizes, const char* name) {
-  TORCH_CHECK(tokens.device() == logits.device() && tokens.scalar_type() == at::kLong && tokens.sizes() == sizes, name,
-              " must be int64 on the logits' device, of shape ", sizes);
-  return tokens.contiguous();
+  TORCH_CHECK_VALUE(at::isIntegralType(tokens.scalar_type(), false), name, " must be integers, not ", tokens.scalar_type());
+  TORCH_CHECK_VALUE(tokens.sizes() == sizes && tokens.device() == logits.device(), name, " must be ", sizes, " on ",
+                    logits.device(), ", not ", tokens.sizes(), " on ", tokens.device());
+  return tokens.to(at::kLong).contiguous();
 }
 
 // ---- log probabilities -----------------------------------------------------------
@@ -225,9 +227,9 @@ tokenLogProbs(const at::Tensor& logits, std::optional<at::Tensor> tokens, double
               int64_t top_k) {
   checkLogits(logits);
   checkTemperature(temperature);
-  TORCH_CHECK(top_k >= 0 && top_k <= kMostTopTokens && top_k <= logits.size(-1), "top_k must be at most ",
-              kMostTopTokens, " and the vocabulary");
-  TORCH_CHECK(tokens.has_value() || entropy || top_k > 0, "nothing is asked for");
+  TORCH_CHECK_VALUE(top_k >= 0 && top_k <= kMostTopTokens && top_k <= logits.size(-1),
+                    "top_k must be from 0 to the vocabulary, ", logits.size(-1), ", and here to ", kMostTopTokens, ", not ", top_k);
+  TORCH_CHECK_VALUE(tokens.has_value() || entropy || top_k > 0, "nothing is asked for: give tokens, entropy=True or top_k");
   c10::cuda::CUDAGuard guard(logits.device());
   if (tokens.has_value()) tokens = checkTokens(*tokens, logits, logits.sizes().slice(0, logits.dim() - 1), "tokens");
   std::tuple<std::optional<at::Tensor>, std::optional<at::Tensor>, std::optional<at::Tensor>, std::optional<at::Tensor>> out;
@@ -253,33 +255,39 @@ tokenLogProbs(const at::Tensor& logits, std::optional<at::Tensor> tokens, double
 }
 
 // ---- distillation ----------------------------------------------------------------
+// `kept`: of every row 4 floats and, for the backward, its tokens' pairs; the number of rows that count, for the mean.
 struct Distillation {
-  at::Tensor loss, stats, merged, count;
+  at::Tensor loss, kept;
+};
+struct Kept {
+  float* count;
+  float* stats;
+  void* merged;
+  Kept(const at::Tensor& kept, int64_t rows)
+      : count(kept.data_ptr<float>()), stats(count + 4), merged(stats + 4 * rows) {}  // 16-byte steps
 };
 
 Distillation distillationForward(const Rows& rows, const at::Tensor& tokens, const at::Tensor& log_probs,
                                  double temperature, bool rest, bool mean, bool keep) {
   const auto fopt = rows.t.options().dtype(at::kFloat);
   const auto stream = c10::cuda::getCurrentCUDAStream();
+  const int64_t n = rows.x.rows, k = tokens.size(-1);
   Distillation out;
-  out.loss = at::empty(rows.t.sizes().slice(0, rows.t.dim() - 1), fopt);
-  out.stats = at::empty({rows.x.rows, 4}, fopt);
-  if (keep) out.merged = at::empty({rows.x.rows, tokens.size(-1), 2}, fopt.dtype(at::kInt));
+  out.kept = at::empty({4 + 4 * n + (keep ? 2 * k * n : 0) + (mean ? n : 0)}, fopt);
+  const Kept kept(out.kept, n);
+  out.loss = mean ? at::empty({}, fopt) : at::empty(rows.t.sizes().slice(0, rows.t.dim() - 1), fopt);
+  float* losses = mean ? kept.stats + 4 * n + (keep ? 2 * k * n : 0) : out.loss.data_ptr<float>();
   DistillationArgs a;
   a.tokens = tokens.data_ptr<int64_t>();
   a.log_probs = log_probs.data_ptr<float>();
-  a.k = (int)tokens.size(-1);
+  a.k = (int)k;
   a.temperature = temperature;
   a.rest = rest;
-  cudaError_t e = launchDistillation(rows.t.data_ptr(), rows.x, a, out.loss.data_ptr<float>(), out.stats.data_ptr<float>(),
-                                     keep ? out.merged.data_ptr() : nullptr, multiprocessors(), stream);
+  cudaError_t e = launchDistillation(rows.t.data_ptr(), rows.x, a, losses, kept.stats, keep ? kept.merged : nullptr,
+                                     multiprocessors(), stream);
   TORCH_CHECK(e == cudaSuccess, "distillation launch failed: ", cudaGetErrorString(e));
   if (mean) {
-    const at::Tensor losses = out.loss;
-    out.loss = at::empty({}, fopt);
-    out.count = at::empty({1}, fopt);
-    e = launchDistillationMean(losses.data_ptr<float>(), out.stats.data_ptr<float>(), rows.x.rows,
-                               out.loss.data_ptr<float>(), out.count.data_ptr<float>(), stream);
+    e = launchDistillationMean(losses, kept.stats, n, out.loss.data_ptr<float>(), kept.count, stream);
     TORCH_CHECK(e == cudaSuccess, "distillation mean launch failed: ", cudaGetErrorString(e));
   }
   return out;
@@ -287,7 +295,7 @@ Distillation distillationForward(const Rows& rows, const at::Tensor& tokens, con
 
 // The gradient of the logits from torch's ops, where its own graph is wanted.
 at::Tensor distillationBackwardGraph(const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& log_probs,
-                                     double temperature, bool rest, const at::Tensor& g, const at::Tensor& count) {
+                                     double temperature, bool rest, bool mean, const at::Tensor& g, const at::Tensor& kept) {
   const at::Tensor z = logits.to(at::kFloat) / temperature;
   const at::Tensor there = tokens.ge(0), bad = tokens.ge(logits.size(-1)).any(-1, true);
   const at::Tensor known = there.logical_and(tokens.lt(logits.size(-1)));
@@ -308,7 +316,7 @@ at::Tensor distillationBackwardGraph(const at::Tensor& logits, const at::Tensor&
   }
   grad = grad.scatter_add(-1, at, -q);
   grad = grad.masked_fill(bad, std::numeric_limits<double>::quiet_NaN());
-  at::Tensor up = count.defined() ? g.to(at::kFloat) / count : g.to(at::kFloat).unsqueeze(-1);
+  const at::Tensor up = mean ? g.to(at::kFloat) / kept.select(0, 0) : g.to(at::kFloat).unsqueeze(-1);
   grad = at::where(counts, grad * (up / temperature), at::zeros_like(grad));
   return grad.to(logits.scalar_type());
 }
@@ -317,26 +325,29 @@ struct DistillationNode : torch::autograd::Function<DistillationNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& tokens,
                             const at::Tensor& log_probs, double temperature, bool rest, bool mean) {
     const Distillation out = distillationForward(rowsOf(logits), tokens, log_probs, temperature, rest, mean, true);
-    ctx->save_for_backward({logits, tokens, log_probs, out.stats, out.merged, out.count});
+    ctx->save_for_backward({logits, tokens, log_probs, out.kept});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["rest"] = rest;
+    ctx->saved_data["mean"] = mean;
     return out.loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &logits = saved[0], &merged = saved[4], &count = saved[5], none;
+    const at::Tensor &logits = saved[0], none;
     const double temperature = ctx->saved_data["temperature"].toDouble();
+    const bool mean = ctx->saved_data["mean"].toBool();
     if (at::GradMode::is_enabled())
-      return {distillationBackwardGraph(logits, saved[1], saved[2], temperature, ctx->saved_data["rest"].toBool(), grads[0], count),
+      return {distillationBackwardGraph(logits, saved[1], saved[2], temperature, ctx->saved_data["rest"].toBool(), mean, grads[0],
+                                        saved[3]),
               none, none, none, none, none};
     c10::cuda::CUDAGuard guard(logits.device());
     Rows rows = rowsOf(logits);
     const at::Tensor grad = gradientFor(rows);
     const auto [g, stride] = perRow(grads[0]);
-    const cudaError_t e = launchDistillationBackward(
-        rows.t.data_ptr(), rows.x, grad.data_ptr(), saved[3].data_ptr<float>(), merged.data_ptr(), (int)merged.size(1),
-        temperature, g.data_ptr<float>(), stride, count.defined() ? count.data_ptr<float>() : nullptr,
-        c10::cuda::getCurrentCUDAStream());
+    const Kept kept(saved[3], rows.x.rows);
+    const cudaError_t e = launchDistillationBackward(rows.t.data_ptr(), rows.x, grad.data_ptr(), kept.stats, kept.merged,
+                                                     (int)saved[1].size(-1), temperature, g.data_ptr<float>(), stride,
+                                                     mean ? kept.count : nullptr, c10::cuda::getCurrentCUDAStream());
     TORCH_CHECK(e == cudaSuccess, "distillation backward launch failed: ", cudaGetErrorString(e));
     return {grad, none, none, none, none, none};
   }
@@ -348,15 +359,18 @@ at::Tensor distillation(const at::Tensor& logits, at::Tensor tokens, at::Tensor 
   checkLogits(logits);
   checkTemperature(temperature);
   const int64_t k = tokens.dim() > 0 ? tokens.size(-1) : 0;
-  TORCH_CHECK(k >= 1 && k <= kMostTeacherTokens, "a row has from 1 to ", kMostTeacherTokens, " teacher tokens");
-  TORCH_CHECK(!rest || logits.size(-1) <= kMostRestVocab, "with the rest the vocabulary is at most ", kMostRestVocab);
+  TORCH_CHECK_VALUE(k >= 1 && k <= kMostTeacherTokens, "a row has from 1 to ", kMostTeacherTokens, " teacher tokens");
+  TORCH_CHECK_VALUE(!rest || logits.size(-1) <= kMostRestVocab, "with the rest the vocabulary is at most ", kMostRestVocab);
   std::vector<int64_t> sizes(logits.sizes().begin(), logits.sizes().end());
   sizes.back() = k;
   c10::cuda::CUDAGuard guard(logits.device());
   tokens = checkTokens(tokens, logits, sizes, "teacher_tokens");
-  TORCH_CHECK(log_probs.device() == logits.device() && log_probs.scalar_type() == at::kFloat && log_probs.sizes() == tokens.sizes(),
-              "teacher_log_probs must be fp32, on the logits' device, of the shape of teacher_tokens");
-  log_probs = log_probs.detach().contiguous();
+  TORCH_CHECK_VALUE(at::isFloatingType(log_probs.scalar_type()) && log_probs.sizes() == tokens.sizes() &&
+                        log_probs.device() == logits.device(),
+                    "teacher_log_probs must be floating-point ", tokens.sizes(), " on ", logits.device(), ", not ",
+                    log_probs.scalar_type(), " ", log_probs.sizes(), " on ", log_probs.device());
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && log_probs.requires_grad()), "teacher_log_probs are constants: detach them");
+  log_probs = (log_probs.requires_grad() ? log_probs.detach() : log_probs).to(at::kFloat).contiguous();
   if (at::GradMode::is_enabled() && logits.requires_grad())
     return DistillationNode::apply(logits, tokens, log_probs, temperature, rest, mean);
   return distillationForward(rowsOf(logits.detach()), tokens, log_probs, temperature, rest, mean, false).loss;

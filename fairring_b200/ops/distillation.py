@@ -34,6 +34,12 @@ def distillation_loss(logits: torch.Tensor, teacher_tokens: torch.Tensor, teache
 
     On the GPU up to 256 tokens a row and, with the rest, 2^20 logits come from the kernel, with the leading
     dimensions in any order and strides; otherwise, and off the GPU, it is made of torch's own operations."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
+    if (_takes(logits) and ordinary(teacher_tokens) and ordinary(teacher_log_probs) and teacher_tokens.dim() > 0
+            and teacher_tokens.shape[-1] <= _C.MOST_TEACHER_TOKENS and not (rest and logits.shape[-1] > _C.MOST_REST_VOCAB)):
+        loss = _C.distillation(logits, teacher_tokens, teacher_log_probs, temperature, rest, reduction == "mean")  # checks them
+        return loss.sum() if reduction == "sum" else loss
     _check_logits(logits, temperature)
     if teacher_tokens.dim() < 1 or teacher_tokens.shape[-1] < 1:
         raise ValueError("teacher_tokens must be [..., k] with at least one token a row")
@@ -44,12 +50,6 @@ def distillation_loss(logits: torch.Tensor, teacher_tokens: torch.Tensor, teache
                          f"{teacher_log_probs.dtype} {tuple(teacher_log_probs.shape)} on {teacher_log_probs.device}")
     if teacher_log_probs.requires_grad and torch.is_grad_enabled():
         raise ValueError("teacher_log_probs are constants: detach them")
-    if reduction not in ("mean", "sum", "none"):
-        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', not {reduction!r}")
-    if (_takes(logits) and ordinary(teacher_tokens) and ordinary(teacher_log_probs) and shape[-1] <= _C.MOST_TEACHER_TOKENS
-            and not (rest and logits.shape[-1] > _C.MOST_REST_VOCAB)):
-        loss = _C.distillation(logits, teacher_tokens, teacher_log_probs.float(), temperature, rest, reduction == "mean")
-        return loss.sum() if reduction == "sum" else loss
     loss, counts = _plain_distillation(logits, teacher_tokens, teacher_log_probs, temperature, rest)
     if reduction == "none":
         return loss

@@ -14,6 +14,9 @@ from .. import _C
 from ._plain import ordinary, plain_calls
 
 
+_TYPES = (torch.bfloat16, torch.float32, torch.float16)
+
+
 class TokenLogProbs(NamedTuple):
     """``None`` where it was not asked for; fp32, token numbers int64."""
 
@@ -40,10 +43,9 @@ def _check_tokens(tokens: torch.Tensor, logits: torch.Tensor, shape, name: str) 
 
 def _takes(logits: torch.Tensor) -> bool:
     """Whether the kernels may be handed the logits."""
-    return (ordinary(logits) and plain_calls() and logits.is_cuda
-            and logits.dtype in (torch.float32, torch.bfloat16, torch.float16)
-            and not (torch.is_inference_mode_enabled() and torch.is_grad_enabled() and logits.requires_grad)
-            and logits.shape[-1] <= 2 ** 31 - 65 and logits.numel() < logits.shape[-1] * 2 ** 31)
+    return (ordinary(logits) and logits.is_cuda and plain_calls() and logits.dtype in _TYPES and logits.dim() > 0
+            and 0 < logits.shape[-1] <= 2 ** 31 - 65 and logits.numel() < logits.shape[-1] * 2 ** 31
+            and not (torch.is_inference_mode_enabled() and logits.requires_grad))
 
 
 def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *, temperature: float = 1.0,
@@ -63,6 +65,8 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *,
     On the GPU the leading dimensions may have any order and strides (a batch without its last position,
     a vocabulary without its padding) as long as a row is contiguous; otherwise the logits are copied.  Up
     to 128 entries come from the kernel; off the GPU and for more it is made of torch's own operations."""
+    if _takes(logits) and (tokens is None or ordinary(tokens)) and top_k <= _C.MOST_TOP_TOKENS:
+        return TokenLogProbs(*_C.token_log_probs(logits, tokens, temperature, entropy, top_k))  # checks what it is given
     _check_logits(logits, temperature)
     if tokens is not None:
         tokens = _check_tokens(tokens, logits, logits.shape[:-1], "tokens")
@@ -70,8 +74,6 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *,
         raise ValueError(f"top_k must be from 0 to the vocabulary, {logits.shape[-1]}, not {top_k}")
     if tokens is None and not entropy and not top_k:
         raise ValueError("nothing is asked for: give tokens, entropy=True or top_k")
-    if _takes(logits) and (tokens is None or ordinary(tokens)) and top_k <= _C.MOST_TOP_TOKENS:
-        return TokenLogProbs(*_C.token_log_probs(logits, tokens, temperature, entropy, top_k))
     return _plain_token_log_probs(logits, tokens, temperature, entropy, top_k)
 
 
