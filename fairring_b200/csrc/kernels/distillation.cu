@@ -16,7 +16,7 @@ using namespace softmax_row;
 
 // What the teacher says of one row, and the student of the tokens that it names.
 struct Teacher {
-  alignas(16) int token[kMostTeacherTokens];  // -1: padding or no token
+  int token[kMostTeacherTokens];  // -1: padding or no token
   float q[kMostTeacherTokens];
   float logit[kMostTeacherTokens];
   bool first[kMostTeacherTokens];  // no entry before it names the same token
@@ -55,12 +55,12 @@ struct LeaveListed {
 
 // Takes the listed tokens' logits out of the sweep: a bit for each column of the slice's vectors, so that the bits of what one
 // thread has of a batch are one word (16 bits of fp32 logits), and a word for the columns outside the vectors.
-template <typename T> struct Marks {
+template <typename T, int kWidth = kThreads> struct Marks {
   static constexpr int E = Vec<T>::kElems, kBits = kBatch * E;
   // Whole batches, and at least one: a row without a vector is swept as a batch of none.
-  static __host__ __device__ __forceinline__ int words(int vecs) {
-    const int batches = (vecs + kBatch * kThreads - 1) / (kBatch * kThreads);
-    return (batches > 0 ? batches : 1) * kThreads * kBits / 32;
+  static constexpr __host__ __device__ __forceinline__ int words(int vecs) {
+    const int batches = (vecs + kBatch * kWidth - 1) / (kBatch * kWidth);
+    return (batches > 0 ? batches : 1) * kWidth * kBits / 32;
   }
   static __device__ __forceinline__ bool loose(const Slice<T>& sl, int col) { return col < sl.firstCol() || col >= sl.lastCol(); }
   static __device__ __forceinline__ unsigned looseBit(const Slice<T>& sl, int col) {
@@ -68,19 +68,19 @@ template <typename T> struct Marks {
   }
   static __device__ __forceinline__ unsigned place(const Slice<T>& sl, int col) {
     const unsigned v = (unsigned)(col - sl.firstCol()) / E, e = (unsigned)(col - sl.firstCol()) % E;
-    return (v / (kBatch * kThreads) * kThreads + v % kThreads) * kBits + v / kThreads % kBatch * E + e;
+    return (v / (kBatch * kWidth) * kWidth + v % kWidth) * kBits + v / kWidth % kBatch * E + e;
   }
 };
-struct RestHook {
+template <int kWidth> struct RestHook {
   const unsigned* bits;
   // Those of what this thread has of batch b.
   template <typename T> __device__ __forceinline__ unsigned listed(int b) const {
-    const int unit = b * kThreads + (int)threadIdx.x;
+    const int unit = b * kWidth + (int)threadIdx.x % kWidth;
     return Marks<T>::kBits == 32 ? bits[unit] : reinterpret_cast<const unsigned short*>(bits)[unit];
   }
   template <typename T> __device__ __forceinline__ float batch(uint4 (&now)[kBatch], bool, int i, const Slice<T>& sl) {
     constexpr int E = Vec<T>::kElems;
-    const unsigned mine = listed<T>((i - sl.v0) / (kBatch * kThreads));
+    const unsigned mine = listed<T>((i - sl.v0) / (kBatch * kWidth));
     if (__any_sync(kAll, mine != 0)) {
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
@@ -128,7 +128,6 @@ __device__ __forceinline__ void loadTeacher(Teacher& te, const Given& given, int
     te.logit[i] = known ? toFloat(row[t]) : 0.f;
     if (known) top = fmaxf(top, value);
   }
-  if (lane < 4 && k + lane < kMostTeacherTokens) te.token[k + lane] = -2;  // behind the last: no token
   outside = __any_sync(kAll, outside);
   top = kRest ? 0.f : warpMax(top);
   if (top == -INFINITY) top = 0.f;
@@ -151,15 +150,33 @@ __device__ __forceinline__ void loadTeacher(Teacher& te, const Given& given, int
   __syncwarp();
 }
 
+// Marks the listed tokens of a row, by one warp; returns the bits of those outside the vectors, and whether a token may be named
+// more than once.
+template <int kWidth, typename T>
+__device__ __forceinline__ unsigned markListed(const Teacher& te, int k, const Slice<T>& sl, unsigned* bits, bool& twice) {
+  unsigned loose = 0;
+  bool again = false;
+  for (int i = threadIdx.x & 31; i < k; i += 32) {
+    const int t = te.token[i];
+    if (t < 0) continue;
+    if (Marks<T, kWidth>::loose(sl, t))
+      loose |= Marks<T, kWidth>::looseBit(sl, t), again = true;  // perhaps: there are few
+    else
+      again |= setBit(bits, Marks<T, kWidth>::place(sl, t));
+  }
+  twice = __any_sync(kAll, again);
+  return __reduce_or_sync(kAll, loose);
+}
+
 // Whether a token is named more than once, by one warp.  Its bit is that of its number's end: where another token had set it, that
-// token is looked for among all.  `bits`: kNameWords of zeros, as they are again afterwards.
+// token is looked for among all.  `bits`: `words` of zeros, a power of two, as they are again afterwards.
 constexpr int kNameWords = 1024;
-__device__ __forceinline__ bool namedTwice(const Teacher& te, int k, unsigned* bits) {
+__device__ __forceinline__ bool namedTwice(const Teacher& te, int k, unsigned* bits, int words) {
   const int lane = threadIdx.x & 31;
   bool twice = false;
   for (int first = 0; first < k; first += 32) {
     const int i = first + lane, t = i < k ? te.token[i] : -1;
-    const bool set = t >= 0 && setBit(bits, t % (32 * kNameWords));
+    const bool set = t >= 0 && setBit(bits, t & (32 * words - 1));
     for (unsigned mask = __ballot_sync(kAll, set); mask != 0; mask &= mask - 1) {
       const int wanted = __shfl_sync(kAll, t, __ffs(mask) - 1);
       unsigned found = 0;
@@ -169,33 +186,28 @@ __device__ __forceinline__ bool namedTwice(const Teacher& te, int k, unsigned* b
   }
   __syncwarp();
   for (int i = lane; i < k; i += 32)
-    if (te.token[i] >= 0) bits[te.token[i] / 32 % kNameWords] = 0;
+    if (te.token[i] >= 0) bits[(te.token[i] >> 5) & (words - 1)] = 0;
   __syncwarp();
   return twice;
 }
 
-// Which entries are the first to name their token, and with `merged` the listed tokens, each once, with the sum of what its entries
-// have, by one warp.  `twice`: a token may be named more than once.
-__device__ __forceinline__ void mergeTeacher(Teacher& te, int k, bool twice, int2* merged) {
-  const int lane = threadIdx.x & 31;
-  for (int i = lane; i < k; i += 32) {
+// Which entries are the first to name their token, and for the backward the listed tokens, each once, with the sum of what its
+// entries have, by one warp.  `twice`: a token may be named more than once.
+__device__ __forceinline__ void mergeTeacher(Teacher& te, int k, bool twice, int2* pairs) {
+  for (int i = threadIdx.x & 31; i < k; i += 32) {
     const int t = te.token[i];
     float q = te.q[i];
     bool first = t >= 0;
     if (twice) {
-      int before = k;
       q = 0.f;
-      for (int j = 0; j < k; j += 4) {  // four at a time
-        const int4 o = *reinterpret_cast<const int4*>(&te.token[j]);
-        if (o.x == t) q += te.q[j], before = min(before, j);
-        if (o.y == t) q += te.q[j + 1], before = min(before, j + 1);
-        if (o.z == t) q += te.q[j + 2], before = min(before, j + 2);
-        if (o.w == t) q += te.q[j + 3], before = min(before, j + 3);
-      }
-      first = first && before == i;
+      for (int j = 0; j < k; ++j)
+        if (te.token[j] == t) {
+          q += te.q[j];
+          first = first && j >= i;
+        }
     }
     te.first[i] = first;
-    if (merged != nullptr) merged[i] = make_int2(first ? t : -1, __float_as_int(q));
+    if (pairs != nullptr) pairs[i] = make_int2(first ? t : -1, __float_as_int(q));
   }
   __syncwarp();
 }
@@ -263,21 +275,24 @@ __device__ __forceinline__ void skipRow(float* loss, float4* stats) {
 template <typename T, bool kRest>
 __global__ void __launch_bounds__(kThreads, 4)
 distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given given, float c, double inv_t,
-                           float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged) {
+                           float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ pairs) {
   namespace cg = cooperative_groups;
   __shared__ Teacher te;
   __shared__ Sums scratch[kWarps], mine;
   __shared__ unsigned loose;
-  extern __shared__ __align__(16) unsigned bits[];
+  extern __shared__ __align__(16) unsigned names[];
+  unsigned* bits = names + kNameWords;  // with the rest
   const cg::cluster_group cluster = cg::this_cluster();
   const int slices = cluster.num_blocks(), rank = cluster.block_rank();
   const int64_t r = blockIdx.x / slices;
   const int tid = threadIdx.x, k = given.k;
   const T* row = rowOf(x, logits, r);
   const Slice<T> sl(row, x.vocab, rank, slices);
-  RestHook hook;
+  RestHook<kThreads> hook;
   hook.bits = bits;
   if (tid == 0) loose = 0;
+  if (rank == 0)
+    for (int i = tid; i < kNameWords; i += kThreads) names[i] = 0;
   if constexpr (kRest)
     for (int i = tid; i < Marks<T>::words(sl.v1 - sl.v0); i += kThreads) bits[i] = 0;
   bool some = false;
@@ -301,15 +316,16 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given give
   Listed l = {};
   if (rank == 0 && tid < 32) {
     loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
-    mergeTeacher(te, k, true, merged != nullptr ? merged + r * k : nullptr);
+    if (kRest || pairs != nullptr)
+      mergeTeacher(te, k, namedTwice(te, k, names, kNameWords), pairs != nullptr ? pairs + r * k : nullptr);
     l = listedOf<kRest>(te, k, c);
   }
   Sums acc;
   if constexpr (kRest) {
-    acc = scan<T, false>(sl, c, hook);
+    acc = scan<T, false, kThreads>(sl, c, hook);
   } else {
     NoHook none;
-    acc = scan<T, false>(sl, c, none);
+    acc = scan<T, false, kThreads>(sl, c, none);
   }
   if (tid < 2 * Vec<T>::kElems) {
     const int col = sl.looseCol(tid);
@@ -330,6 +346,60 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given give
   if (tid == 0) finishRow<kRest>(l, acc, te.outside, c, inv_t, loss + r, stats + r);
 }
 
+// Many short rows: one per warp.
+template <typename T> struct ShortRow {
+  Teacher teacher;
+  static constexpr int kWords = Marks<T, 32>::words(kShortBytes / 16);
+  unsigned bits[kWords];  // a power of two, and as many bits as a short row has tokens
+};
+template <typename T, bool kRest>
+__global__ void __launch_bounds__(kThreads, 4)
+distillation_short_kernel(const T* __restrict__ logits, LogitRows x, Given given, float c, double inv_t, float* __restrict__ loss,
+                          float4* __restrict__ stats, int2* __restrict__ pairs) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  ShortRow<T>& mine = reinterpret_cast<ShortRow<T>*>(dynamic)[threadIdx.x >> 5];
+  Teacher& te = mine.teacher;
+  const int lane = threadIdx.x & 31, k = given.k;
+  const int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (r >= x.rows) return;
+  if (!countsAtAll<kRest>(given, r)) {
+    if (lane == 0) skipRow(loss + r, stats + r);
+    return;
+  }
+  const T* row = rowOf(x, logits, r);
+  const Slice<T> sl(row, x.vocab, 0, 1);
+  loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
+  for (int i = lane; i < ShortRow<T>::kWords; i += 32) mine.bits[i] = 0;
+  __syncwarp();
+  unsigned left_out = 0;
+  bool twice = false;
+  if (kRest)
+    left_out = markListed<32>(te, k, sl, mine.bits, twice);
+  else if (pairs != nullptr)
+    twice = namedTwice(te, k, mine.bits, ShortRow<T>::kWords);
+  if (kRest || pairs != nullptr) mergeTeacher(te, k, twice, pairs != nullptr ? pairs + r * k : nullptr);
+  Sums acc;
+  if constexpr (kRest) {
+    RestHook<32> hook;
+    hook.bits = mine.bits;
+    acc = scan<T, false, 32>(sl, c, hook);
+  } else {
+    NoHook none;
+    acc = scan<T, false, 32>(sl, c, none);
+  }
+  const Listed l = listedOf<kRest>(te, k, c);
+  const int col = lane < 2 * Vec<T>::kElems && !(left_out >> lane & 1u) ? sl.looseCol(lane) : -1;
+  if (col >= 0) acc.add<false>(toFloat(row[col]), c);
+  acc = warpSums<false>(acc, c);
+  if (!acc.settle<false>(c)) {
+    if constexpr (kRest)
+      acc = warpAgain<T, false>(row, x.vocab, c, LeaveListed{&te, k});
+    else
+      acc = warpAgain<T, false>(row, x.vocab, c, LeaveNone());
+  }
+  if (lane == 0) finishRow<kRest>(l, acc, te.outside, c, inv_t, loss + r, stats + r);
+}
+
 // Many rows: the blocks stay.  With the rest the fetching warp marks the listed tokens of a row while the row before it is
 // swept, in place of those of the row before that.
 // A row that needs no more than finishRow(), which is done for 32 of them at once.
@@ -345,9 +415,9 @@ struct DistillRows {
   Teacher teacher[kSlots];
   unsigned loose[kSlots];  // the listed columns outside the vectors
   Pending pending[32];
-  alignas(16) unsigned bits[1];  // with the rest twice, else once, as many words as the kernel is told
+  alignas(16) unsigned bits[1];  // kNameWords; with the rest, twice as many words as the kernel is told
 };
-template <typename T> struct RestRowsHook : RestHook {
+template <typename T> struct RestRowsHook : RestHook<kThreads> {
   const unsigned* all;
   HandOver* hand;
   int words_a_row, turn = 1;
@@ -359,7 +429,7 @@ template <typename T> struct RestRowsHook : RestHook {
   __device__ __forceinline__ void end() {}
   __device__ __forceinline__ void arrived(uint4* place, int b) {
     constexpr int E = Vec<T>::kElems;
-    for (unsigned mine = listed<T>(b); mine != 0; mine &= mine - 1) {
+    for (unsigned mine = this->template listed<T>(b); mine != 0; mine &= mine - 1) {
       const int at = __ffs(mine) - 1;
       fromFloat(reinterpret_cast<T*>(place + at / E * kThreads) + at % E, -INFINITY);
     }
@@ -369,12 +439,12 @@ template <typename T> struct RestRowsHook : RestHook {
 template <typename T, bool kRest>
 __global__ void __launch_bounds__(kRowThreads, 3)
 distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Given given, float c, double inv_t,
-                         float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ merged, int words, int rows_a_block) {
+                         float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ pairs, int words, int rows_a_block) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   DistillRows& shared = *reinterpret_cast<DistillRows*>(dynamic);
   HandOver& hand = shared.hand;
   if (threadIdx.x == 0) hand.init();
-  for (int i = threadIdx.x; i < words * (kRest ? 2 : 1); i += kRowThreads) shared.bits[i] = 0;
+  for (int i = threadIdx.x; i < (kRest ? 2 * words : kNameWords); i += kRowThreads) shared.bits[i] = 0;
   __syncthreads();
   if (threadIdx.x < kThreads) {
     if constexpr (kRest) {
@@ -408,42 +478,29 @@ distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Given given,
           const T* row = rowOf(x, logits, r);
           if (!kRest) loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
           bool twice = false;
-          {
-            if constexpr (kRest) {
-              unsigned* bits = shared.bits + (fetched & 1) * words;
-              if (fetched >= 2) {  // swept: its marks go
-                hand.wait(&hand.full[before.slot], before.parity);
-                const Slice<T> sl(rowOf(x, logits, marked_before), x.vocab, 0, 1);
-                const Teacher& old = shared.teacher[before.slot];
-                for (int i = lane; i < k; i += 32)
-                  if (old.token[i] >= 0 && !Marks<T>::loose(sl, old.token[i])) bits[Marks<T>::place(sl, old.token[i]) >> 5] = 0;
-                before.next();
-                __syncwarp();
-              }
-              marked_before = marked;
-              marked = r;
-              const Slice<T> sl(row, x.vocab, 0, 1);
-              unsigned loose = 0;
-              for (int i = lane; i < k; i += 32) {
-                const int t = te.token[i];
-                if (t < 0) continue;
-                if (Marks<T>::loose(sl, t))
-                  loose |= Marks<T>::looseBit(sl, t), twice = true;  // perhaps: there are few
-                else
-                  twice |= setBit(bits, Marks<T>::place(sl, t));
-              }
-              loose = __reduce_or_sync(kAll, loose);
-              if (lane == 0) {
-                shared.loose[at.slot] = loose;
-                barrierArrive(&hand.marked[at.slot]);
-              }
-              ++fetched;
-            } else if (merged != nullptr) {
-              twice = namedTwice(te, k, shared.bits);
+          if constexpr (kRest) {
+            unsigned* bits = shared.bits + (fetched & 1) * words;
+            if (fetched >= 2) {  // swept: its marks go
+              hand.wait(&hand.full[before.slot], before.parity);
+              const Slice<T> sl(rowOf(x, logits, marked_before), x.vocab, 0, 1);
+              const Teacher& old = shared.teacher[before.slot];
+              for (int i = lane; i < k; i += 32)
+                if (old.token[i] >= 0 && !Marks<T>::loose(sl, old.token[i])) bits[Marks<T>::place(sl, old.token[i]) >> 5] = 0;
+              before.next();
+              __syncwarp();
             }
+            marked_before = marked;
+            marked = r;
+            const unsigned loose = markListed<kThreads>(te, k, Slice<T>(row, x.vocab, 0, 1), bits, twice);
+            if (lane == 0) {
+              shared.loose[at.slot] = loose;
+              barrierArrive(&hand.marked[at.slot]);
+            }
+            ++fetched;
+          } else if (pairs != nullptr) {
+            twice = namedTwice(te, k, shared.bits, kNameWords);
           }
-          if (kRest || merged != nullptr)
-            mergeTeacher(te, k, kRest ? __any_sync(kAll, twice) : twice, merged != nullptr ? merged + (int64_t)r * k : nullptr);
+          if (kRest || pairs != nullptr) mergeTeacher(te, k, twice, pairs != nullptr ? pairs + (int64_t)r * k : nullptr);
         });
     return;
   }
@@ -503,7 +560,7 @@ distillation_mean_kernel(const float* __restrict__ loss, const float4* __restric
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, const float4* __restrict__ stats,
-                        const int2* __restrict__ merged, int k, float c, float inv_t, const float* __restrict__ upstream,
+                        const int2* __restrict__ pairs, int k, float c, float inv_t, const float* __restrict__ upstream,
                         int64_t stride, const float* __restrict__ count, int64_t pieces_total, int pieces) {
   constexpr int E = Vec<T>::kElems, U = kBatch;
   for (int64_t w = blockIdx.x; w < pieces_total; w += gridDim.x) {
@@ -524,7 +581,7 @@ distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, cons
     int2 mine = make_int2(-1, 0);
     float logit = 0.f;
     if (counts && (int)threadIdx.x < k) {
-      mine = merged[r * k + threadIdx.x];
+      mine = pairs[r * k + threadIdx.x];
       const int v = (mine.x - parts.head) / E / (U * kThreads);
       const bool vector = mine.x >= parts.head && mine.x < parts.head + parts.nvec * E;
       if (mine.x >= 0 && (vector ? v : 0) != piece) mine.x = -1;
@@ -563,42 +620,45 @@ distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, cons
 }
 
 template <typename T, bool kRest>
-cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float4* stats, int2* merged,
+cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float4* stats, int2* pairs,
                       int sm_count, cudaStream_t stream) {
   const float c = (float)(1.4426950408889634 / a.temperature);
   const double inv_t = 1.0 / a.temperature;
   const Given given{a.tokens, a.log_probs, a.k};
-  const int words = kRest ? Marks<T>::words(x.vocab / Vec<T>::kElems) : kNameWords;
-  const size_t stay = sizeof(DistillRows) + (kRest ? 2 : 1) * (size_t)words * 4;
+  if (shortRows(x, sizeof(T), sm_count))
+    return launchShort(distillation_short_kernel<T, kRest>, x.rows, kWarps * sizeof(ShortRow<T>), stream, logits, x, given, c, inv_t,
+                       loss, stats, pairs);
+  const int words = kRest ? Marks<T>::words(x.vocab / Vec<T>::kElems) : 0;
+  const size_t stay = sizeof(DistillRows) + (kRest ? 2 * (size_t)words : kNameWords) * 4;
   // Two blocks of the form that stays have to fit on a multiprocessor; up to 65536 tokens of 16 bits three do.
   if (manyRows(x.rows, sm_count) && stay <= 112 * 1024) {
-    const int rows_a_block = rowsABlock(x, sizeof(T));
+    const int rows_a_block = rowsABlock(x, sizeof(T), sm_count);
     return launchRows(distillation_rows_kernel<T, kRest>, x.rows, rows_a_block, stay, stream, logits, x, given, c, inv_t, loss, stats,
-                      merged, words, rows_a_block);
+                      pairs, words, rows_a_block);
   }
   const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
-  const size_t shared = kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) * 4 : 0;
+  const size_t shared = 4 * (kNameWords + (kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) : 0));
   if (shared > 32 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(distillation_slices_kernel<T, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)shared);
     if (e != cudaSuccess) return e;
   }
   return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, shared, stream, logits, x, given, c, inv_t, loss,
-                      stats, merged);
+                      stats, pairs);
 }
 
 template <typename T>
 cudaError_t forwardOf(const void* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float* stats,
-                      void* merged, int sm_count, cudaStream_t stream) {
+                      void* pairs_, int sm_count, cudaStream_t stream) {
   const T* data = static_cast<const T*>(logits);
   float4* st = reinterpret_cast<float4*>(stats);
-  int2* pairs = static_cast<int2*>(merged);
+  int2* pairs = static_cast<int2*>(pairs_);
   return a.rest ? forwardOf<T, true>(data, x, a, loss, st, pairs, sm_count, stream)
                 : forwardOf<T, false>(data, x, a, loss, st, pairs, sm_count, stream);
 }
 
 template <typename T>
-cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const float* stats, const void* merged, int k,
+cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const float* stats, const void* pairs, int k,
                        double temperature, const float* upstream, int64_t stride, const float* count, cudaStream_t stream) {
   constexpr int per_piece = kThreads * kBatch * Vec<T>::kElems;
   const int pieces = (int)(((int64_t)x.vocab + per_piece - 1) / per_piece);
@@ -606,7 +666,7 @@ cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const
   const unsigned blocks = (unsigned)(total < (1 << 30) ? total : (1 << 30));
   distillation_bwd_kernel<T><<<blocks, kThreads, 0, stream>>>(
       static_cast<const T*>(logits), x, static_cast<T*>(grad), reinterpret_cast<const float4*>(stats),
-      static_cast<const int2*>(merged), k, (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature), upstream,
+      static_cast<const int2*>(pairs), k, (float)(1.4426950408889634 / temperature), (float)(1.0 / temperature), upstream,
       stride, count, total, pieces);
   noteLocalLaunch();
   return cudaGetLastError();
@@ -615,14 +675,14 @@ cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const
 }  // namespace
 
 cudaError_t launchDistillation(const void* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float* stats,
-                               void* merged, int sm_count, cudaStream_t stream) {
+                               void* pairs, int sm_count, cudaStream_t stream) {
   if (x.rows <= 0) return cudaSuccess;
   if (x.vocab <= 0 || x.rows > INT32_MAX || a.k <= 0 || a.k > kMostTeacherTokens || (a.rest && x.vocab > kMostRestVocab))
     return cudaErrorInvalidValue;
   switch (x.type) {
-    case LogitType::kBFloat16: return forwardOf<__nv_bfloat16>(logits, x, a, loss, stats, merged, sm_count, stream);
-    case LogitType::kHalf: return forwardOf<__half>(logits, x, a, loss, stats, merged, sm_count, stream);
-    default: return forwardOf<float>(logits, x, a, loss, stats, merged, sm_count, stream);
+    case LogitType::kBFloat16: return forwardOf<__nv_bfloat16>(logits, x, a, loss, stats, pairs, sm_count, stream);
+    case LogitType::kHalf: return forwardOf<__half>(logits, x, a, loss, stats, pairs, sm_count, stream);
+    default: return forwardOf<float>(logits, x, a, loss, stats, pairs, sm_count, stream);
   }
 }
 
@@ -634,7 +694,7 @@ cudaError_t launchDistillationMean(const float* loss, const float* stats, int64_
 }
 
 cudaError_t launchDistillationBackward(const void* logits, const LogitRows& x, void* grad, const float* stats,
-                                       const void* merged, int k, double temperature, const float* upstream, int64_t stride,
+                                       const void* pairs, int k, double temperature, const float* upstream, int64_t stride,
                                        const float* count, cudaStream_t stream) {
   if (x.rows <= 0) return cudaSuccess;
   if (x.vocab <= 0 || x.rows > INT32_MAX || k <= 0 || k > kMostTeacherTokens) return cudaErrorInvalidValue;
@@ -642,11 +702,11 @@ cudaError_t launchDistillationBackward(const void* logits, const LogitRows& x, v
   if ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad)) & 15u) return cudaErrorMisalignedAddress;
   switch (x.type) {
     case LogitType::kBFloat16:
-      return backwardOf<__nv_bfloat16>(logits, x, grad, stats, merged, k, temperature, upstream, stride, count, stream);
+      return backwardOf<__nv_bfloat16>(logits, x, grad, stats, pairs, k, temperature, upstream, stride, count, stream);
     case LogitType::kHalf:
-      return backwardOf<__half>(logits, x, grad, stats, merged, k, temperature, upstream, stride, count, stream);
+      return backwardOf<__half>(logits, x, grad, stats, pairs, k, temperature, upstream, stride, count, stream);
     default:
-      return backwardOf<float>(logits, x, grad, stats, merged, k, temperature, upstream, stride, count, stream);
+      return backwardOf<float>(logits, x, grad, stats, pairs, k, temperature, upstream, stride, count, stream);
   }
 }
 

@@ -179,8 +179,8 @@ cudaError_t launchTokenLogProbsBackward(const void* logits, const LogitRows& x, 
                                         cudaStream_t stream);
 
 // Divergence of the rows' softmax from a teacher's `k` log probabilities a row; a negative token is padding.  `rest`:
-// what they leave of the probability, if it is more than the rounding of fp32 log probabilities, is one more class.  `stats` (4 floats a row) and `merged` (k pairs of token and
-// probability a row) are for the backward; `merged` may be null.
+// what they leave of the probability, if it is more than the rounding of fp32 log probabilities, is one more class.  `stats` (4 floats a row) and `pairs` (k of token and
+// probability a row) are for the backward; `pairs` may be null.
 constexpr int kMostTeacherTokens = 256;
 constexpr int kMostRestVocab = 1 << 20;
 constexpr double kLeastRest = 1.0 / (1 << 20);
@@ -192,13 +192,13 @@ struct DistillationArgs {
   bool rest;
 };
 cudaError_t launchDistillation(const void* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float* stats,
-                               void* merged, int sm_count, cudaStream_t stream);
+                               void* pairs, int sm_count, cudaStream_t stream);
 // *mean = sum of `loss` / *count, *count = number of rows that count, at least 1.
 cudaError_t launchDistillationMean(const float* loss, const float* stats, int64_t rows, float* mean, float* count,
                                    cudaStream_t stream);
 // The gradient, scaled by upstream[row * stride] / *count (count may be null); `grad` as above.
 cudaError_t launchDistillationBackward(const void* logits, const LogitRows& x, void* grad, const float* stats,
-                                       const void* merged, int k, double temperature, const float* upstream, int64_t stride,
+                                       const void* pairs, int k, double temperature, const float* upstream, int64_t stride,
                                        const float* count, cudaStream_t stream);
 
 uint64_t localLaunchCountImpl();

@@ -290,9 +290,9 @@ struct NoHook {
   }
 };
 
-// This thread's share of the slice.  All threads of a block go through the same number of batches.  The next batch is on its
+// This thread's share of the slice, by kWidth threads that all go through the same number of batches.  The next batch is on its
 // way while this one is used.
-template <typename T, bool kEntropy, class Hook>
+template <typename T, bool kEntropy, int kWidth, class Hook>
 __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
   constexpr int U = kBatch;
   constexpr uint32_t w = Vec<T>::kMinusInf;
@@ -301,18 +301,18 @@ __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
   auto fetch = [&](int i) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      raw[u] = i + u * kThreads < sl.v1 ? __ldg(vecs + i + u * kThreads) : make_uint4(w, w, w, w);
+      raw[u] = i + u * kWidth < sl.v1 ? __ldg(vecs + i + u * kWidth) : make_uint4(w, w, w, w);
   };
   ThreadSums acc(c);
-  const int batches = (sl.v1 - sl.v0 + U * kThreads - 1) / (U * kThreads);
-  int i = sl.v0 + (int)threadIdx.x;
+  const int batches = (sl.v1 - sl.v0 + U * kWidth - 1) / (U * kWidth);
+  int i = sl.v0 + (int)threadIdx.x % kWidth;
   fetch(i);
-  for (int b = 0; b < batches; ++b, i += U * kThreads) {
+  for (int b = 0; b < batches; ++b, i += U * kWidth) {
     uint4 now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = raw[u];
-    fetch(i + U * kThreads);
-    acc.add<T, kEntropy, false>(now, hook.batch(now, b == 0, i, sl), (sl.v1 - (i & ~31) + kThreads - 1) / kThreads, c);
+    fetch(i + U * kWidth);
+    acc.add<T, kEntropy, false>(now, hook.batch(now, b == 0, i, sl), (sl.v1 - (i - (int)(threadIdx.x & 31)) + kWidth - 1) / kWidth, c);
   }
   return acc.sums();
 }
@@ -567,10 +567,12 @@ struct HandOver {
 
 using Ring = uint4[kDepth][kBatch][kThreads];
 
-// How many rows a block of the grid stands for: as many as make up 64 KB, so that asking for them does not cost more than they do.
-inline int rowsABlock(const LogitRows& x, int elem_size) {
-  const int64_t n = (65536 + (int64_t)x.vocab * elem_size - 1) / ((int64_t)x.vocab * elem_size);
-  return n < 32 ? (int)n : 32;
+// How many rows a block of the grid stands for: as many as make up 64 KB, so that asking for them does not cost more than they do,
+// but so few that there are four blocks for each of those that stay.
+inline int rowsABlock(const LogitRows& x, int elem_size, int sm_count) {
+  const int64_t by_size = (65536 + (int64_t)x.vocab * elem_size - 1) / ((int64_t)x.vocab * elem_size), by_rows = x.rows / (12 * sm_count);
+  const int64_t n = by_size < by_rows ? by_size : by_rows;
+  return n < 1 ? 1 : n < 32 ? (int)n : 32;
 }
 
 // The fetching warp's part.  `counts(r)`, by one lane, says that a row does not count as far as that is seen at once, else skip(r), by
@@ -721,6 +723,20 @@ cudaError_t launchRows(void (*kernel)(Params...), int64_t rows, int rows_a_block
 
 // Whether rows are many enough for that: several for each of the blocks that stay.
 inline bool manyRows(int64_t rows, int sm_count) { return rows >= kManyRows * (int64_t)sm_count; }
+
+// ---- many short rows -------------------------------------------------------------
+// Up to 16 KB a row is one warp's, which sweeps and finishes it: no thread waits for another warp, and a multiprocessor has 32 rows on
+// the way.
+constexpr int kShortBytes = 16384;
+inline bool shortRows(const LogitRows& x, int elem_size, int sm_count) {
+  return (int64_t)x.vocab * elem_size <= kShortBytes && manyRows(x.rows, sm_count);
+}
+template <typename... Params, typename... Args>
+cudaError_t launchShort(void (*kernel)(Params...), int64_t rows, size_t shared, cudaStream_t stream, Args... args) {
+  kernel<<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, shared, stream>>>(Params(args)...);
+  noteLocalLaunch();
+  return cudaGetLastError();
+}
 
 }  // namespace softmax_row
 }  // namespace fairring

@@ -385,11 +385,11 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
     TopHook hook;
     hook.groups = &top->groups;
     if (threadIdx.x == 0) top->work.listed = top->work.queued = 0;
-    acc = scan<T, kEntropy>(sl, c, hook);
+    acc = scan<T, kEntropy, kThreads>(sl, c, hook);
     hook.end();
   } else {
     NoHook none;
-    acc = scan<T, kEntropy>(sl, c, none);
+    acc = scan<T, kEntropy, kThreads>(sl, c, none);
   }
   if (threadIdx.x < 2 * Vec<T>::kElems) {
     const int col = sl.looseCol(threadIdx.x);
@@ -406,6 +406,30 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
   if (!acc.template settle<kEntropy>(c)) acc = blockAgain<T, kEntropy>(sl.row, x.vocab, c, scratch, LeaveNone());
   if (threadIdx.x == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
   if constexpr (kTop) out.largest<BlockGroup>(r, acc, top->work.best, inv_t);
+}
+
+// Many short rows: one per warp.
+template <typename T, bool kEntropy>
+__global__ void __launch_bounds__(kThreads, 4)
+token_log_probs_short_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (r >= x.rows) return;
+  const int64_t t = out.tokens != nullptr ? out.tokens[r] : 0;
+  if (t < 0) {
+    if (lane == 0) out.skipped(r);
+    return;
+  }
+  const Slice<T> sl(rowOf(x, logits, r), x.vocab, 0, 1);
+  const bool known = t < x.vocab;
+  const float logit = known ? toFloat(sl.row[t]) : 0.f;
+  NoHook none;
+  Sums acc = scan<T, kEntropy, 32>(sl, c, none);
+  const int col = lane < 2 * Vec<T>::kElems ? sl.looseCol(lane) : -1;
+  if (col >= 0) acc.add<kEntropy>(toFloat(sl.row[col]), c);
+  acc = warpSums<kEntropy>(acc, c);
+  if (!acc.template settle<kEntropy>(c)) acc = warpAgain<T, kEntropy>(sl.row, x.vocab, c, LeaveNone());
+  if (lane == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
 }
 
 // Many rows: the blocks stay.
@@ -520,8 +544,10 @@ token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restr
 template <typename T, bool kEntropy>
 cudaError_t forwardOf(const T* logits, const LogitRows& x, const Outputs& out, double temperature, int sm_count, cudaStream_t stream) {
   const float inv_t = (float)(1.0 / temperature), c = (float)(1.4426950408889634 / temperature);
+  if (out.k == 0 && shortRows(x, sizeof(T), sm_count))
+    return launchShort(token_log_probs_short_kernel<T, kEntropy>, x.rows, 0, stream, logits, x, out, c, inv_t);
   if (out.k == 0 && manyRows(x.rows, sm_count)) {
-    const int rows_a_block = rowsABlock(x, sizeof(T));
+    const int rows_a_block = rowsABlock(x, sizeof(T), sm_count);
     return launchRows(token_log_probs_rows_kernel<T, kEntropy>, x.rows, rows_a_block, sizeof(Rows), stream, logits, x, out, c, inv_t,
                       rows_a_block);
   }

@@ -262,9 +262,9 @@ struct Distillation {
 struct Kept {
   float* count;
   float* stats;
-  void* merged;
+  void* pairs;
   Kept(const at::Tensor& kept, int64_t rows)
-      : count(kept.data_ptr<float>()), stats(count + 4), merged(stats + 4 * rows) {}  // 16-byte steps
+      : count(kept.data_ptr<float>()), stats(count + 4), pairs(stats + 4 * rows) {}  // 16-byte steps
 };
 
 Distillation distillationForward(const Rows& rows, const at::Tensor& tokens, const at::Tensor& log_probs,
@@ -283,7 +283,7 @@ Distillation distillationForward(const Rows& rows, const at::Tensor& tokens, con
   a.k = (int)k;
   a.temperature = temperature;
   a.rest = rest;
-  cudaError_t e = launchDistillation(rows.t.data_ptr(), rows.x, a, losses, kept.stats, keep ? kept.merged : nullptr,
+  cudaError_t e = launchDistillation(rows.t.data_ptr(), rows.x, a, losses, kept.stats, keep ? kept.pairs : nullptr,
                                      multiprocessors(), stream);
   TORCH_CHECK(e == cudaSuccess, "distillation launch failed: ", cudaGetErrorString(e));
   if (mean) {
@@ -345,7 +345,7 @@ struct DistillationNode : torch::autograd::Function<DistillationNode> {
     const at::Tensor grad = gradientFor(rows);
     const auto [g, stride] = perRow(grads[0]);
     const Kept kept(saved[3], rows.x.rows);
-    const cudaError_t e = launchDistillationBackward(rows.t.data_ptr(), rows.x, grad.data_ptr(), kept.stats, kept.merged,
+    const cudaError_t e = launchDistillationBackward(rows.t.data_ptr(), rows.x, grad.data_ptr(), kept.stats, kept.pairs,
                                                      (int)saved[1].size(-1), temperature, g.data_ptr<float>(), stride,
                                                      mean ? kept.count : nullptr, c10::cuda::getCurrentCUDAStream());
     TORCH_CHECK(e == cudaSuccess, "distillation backward launch failed: ", cudaGetErrorString(e));

@@ -79,8 +79,8 @@ def test_every_row_length(rows, vocab, k, rest, dtype):
         assert loss[2] == 0 and not grad[2].any()
 
 
-# rows that are taken by blocks that stay
-@pytest.mark.parametrize("vocab,k", [(7, 3), (264, 256), (1001, 5), (8193, 64), (20011, 33)])
+# rows of a warp each, and rows that are taken by blocks that stay
+@pytest.mark.parametrize("vocab,k", [(7, 3), (264, 256), (1001, 5), (4099, 100), (8192, 128), (8193, 64), (20011, 33)])
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_many_rows(vocab, k, rest, dtype):
@@ -89,6 +89,14 @@ def test_many_rows(vocab, k, rest, dtype):
     tokens[950:1000, 1:] = tokens[950:1000, :1]  # one token all over
     tokens[1299, :-1] = -1  # only the last entry
     _check(x, tokens, given - 0.2 if rest else given, 1.3, rest)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_several_rows_a_block(rest):
+    x, tokens, given = _case(4001, 8200, 6, torch.float32)
+    tokens[500:1500] = -1
+    tokens[torch.rand(4001, device="cuda", generator=_gen(3)) < 0.3] = -100
+    _check(x, tokens, given - 0.2 if rest else given, 1.0, rest)
 
 
 @pytest.mark.parametrize("temperature", [0.5, 2.0])

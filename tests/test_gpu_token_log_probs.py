@@ -63,7 +63,7 @@ def _check(logits, tokens, temperature=1.0, entropy=True):
 # one thread's worth, remainders on both sides of the 16-byte vectors, one batch of a block (256 x 4 vectors) and the
 # next; 19 rows are cut into slices from 512 vectors a slice on, 400 rows are not; 1300 rows are taken by blocks that stay
 @pytest.mark.parametrize("rows", [1, 19, 400, 1300])
-@pytest.mark.parametrize("vocab", [1, 7, 8, 9, 1000, 1001, 4096, 8191, 8192, 8193, 16385, 32776, 50265])
+@pytest.mark.parametrize("vocab", [1, 7, 8, 9, 1000, 1001, 4096, 4097, 8191, 8192, 8193, 16385, 32776, 50265])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_every_row_length(rows, vocab, dtype):
     logits = _logits(rows, vocab, dtype)
@@ -208,17 +208,18 @@ def test_views():
     _check(_logits(1, 1003, torch.float32)[0], torch.tensor(5, device="cuda"))  # one row without a leading dimension
 
 
+# a row per warp; several rows per block of those that stay; one
+@pytest.mark.parametrize("rows,vocab", [(20000, 264), (4001, 8200), (1500, 17000)])
 @pytest.mark.parametrize("share", [0.0, 0.02, 0.5, 0.99, 1.0])
-def test_rows_that_do_not_count_among_many(share):
-    """Whole runs of 32 rows of a block without one that counts, and the last rows of all."""
+def test_rows_that_do_not_count_among_many(rows, vocab, share):
+    """Whole runs of rows of a block without one that counts, and the last rows of all."""
     from fairring_b200.ops import token_log_probs
 
-    rows, vocab = 20000, 264
     gen = _gen(8)
     logits = _logits(rows, vocab, torch.float32)
     tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=gen)
     tokens[torch.rand(rows, device="cuda", generator=gen) < share] = -100
-    tokens[:5000] = -1
+    tokens[: rows // 4] = -1
     logits[tokens < 0] = float("nan")
     _check(logits.nan_to_num(), tokens)
     got = token_log_probs(logits, tokens, entropy=True, top_k=3)
