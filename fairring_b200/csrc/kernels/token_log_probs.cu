@@ -223,60 +223,66 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
 #pragma unroll
   for (int w = 1; w < kGroupWarps; ++w) bound = fminf(bound, work.bound[w]);
   bound = fmaxf(bound, -FLT_MAX);  // minus infinity is left to the other way
+  // A thread's groups side by side in the queue, those of a warp after one addition to its length.
+  unsigned pass = 0;
 #pragma unroll
-  for (int j = 0; j < kColumns; ++j)
+  for (int j = 0; j < kColumns * kGroups; ++j) pass |= value[j] >= bound ? 1u << j : 0u;
+  int pos = __popc(pass);
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const bool pass = value[j * kGroups + g] >= bound;
-      const unsigned votes = __ballot_sync(kAll, pass);
-      if (votes == 0) continue;
-      unsigned pos = 0;
-      if (lane == 0) pos = atomicAdd(&work.queued, (unsigned)__popc(votes));
-      pos = __shfl_sync(kAll, pos, 0) + __popc(votes & ((1u << lane) - 1u));
-      if (pass && pos < kQueue) work.queue[pos] = g * kThreads + tid + j * G::kSize;
-    }
+  for (int o = 1; o < 32; o *= 2) {
+    const int below = __shfl_up_sync(kAll, pos, o);
+    if (lane >= o) pos += below;
+  }
+  int at = 0;
+  if (lane == 31) at = atomicAdd(&work.queued, (unsigned)pos);
+  pos += __shfl_sync(kAll, at, 31) - __popc(pass);
+  for (; pass != 0; pass &= pass - 1, ++pos) {
+    const int j = __ffs(pass) - 1;
+    if (pos < kQueue) work.queue[pos] = j % kGroups * kThreads + tid + j / kGroups * G::kSize;
+  }
   G::sync();
-  const int queued = work.queued, vecs_each = kBatch * span;
+  const int queued = work.queued;
   const bool fits = queued <= kQueue;
   const uint4* all = reinterpret_cast<const uint4*>(sl.row + sl.head);
-  constexpr int kAhead = 4;
-  const int items = fits ? queued * vecs_each : 0;
-  for (int first = 0; first < items; first += kAhead * G::kSize) {
-    uint4 raw[kAhead];
-    int at[kAhead];
+  // kBatch threads a group, one for each of the vectors that a batch has of it; two rounds of groups at once.
+  constexpr int kRound = G::kSize / kBatch, kAhead = 2;
+  for (int first = 0; first < queued && fits; first += kAhead * kRound)
+    for (int batch = 0; batch < span; ++batch) {
+      uint4 raw[kAhead];
+      int vec[kAhead];
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-      const int j = first + s * G::kSize + tid;
-      at[s] = sl.v1;
-      if (j < items) {
-        const int id = work.queue[j / vecs_each];
-        at[s] = sl.v0 + id / kThreads * vecs_each * kThreads + j % vecs_each * kThreads + id % kThreads;
-      }
-      constexpr uint32_t w = Vec<T>::kMinusInf;
-      raw[s] = at[s] < sl.v1 ? all[at[s]] : make_uint4(w, w, w, w);  // swept not long ago: from L2
-    }
-#pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-      if (first + s * G::kSize >= items) break;
-      float2 v[E / 2];
-      Vec<T>::get(raw[s], v);
-      unsigned mask = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) mask |= (e & 1 ? v[e / 2].y : v[e / 2].x) >= bound ? 1u << e : 0u;
-      for (;;) {  // a value of every lane that has one
-        const unsigned votes = __ballot_sync(kAll, mask != 0);
-        if (votes == 0) break;
-        unsigned pos = 0;
-        if (lane == 0) pos = atomicAdd(&work.listed, (unsigned)__popc(votes));
-        pos = __shfl_sync(kAll, pos, 0) + __popc(votes & ((1u << lane) - 1u));
-        if (mask != 0 && pos < kList) {
-          const int col = sl.head + at[s] * E + __ffs(mask) - 1;
-          work.list[pos] = entryOf(toFloat(sl.row[col]), col);
+      for (int s = 0; s < kAhead; ++s) {
+        const int q = first + s * kRound + tid / kBatch;
+        vec[s] = sl.v1;
+        if (q < queued) {
+          const int id = work.queue[q];
+          vec[s] = sl.v0 + ((id / kThreads * span + batch) * kBatch + tid % kBatch) * kThreads + id % kThreads;
         }
-        mask &= mask - 1;
+        constexpr uint32_t w = Vec<T>::kMinusInf;
+        raw[s] = vec[s] < sl.v1 ? all[vec[s]] : make_uint4(w, w, w, w);  // swept not long ago: from L2
+      }
+#pragma unroll
+      for (int s = 0; s < kAhead; ++s) {
+        if (first + s * kRound >= queued) break;
+        float2 v[E / 2];
+        Vec<T>::get(raw[s], v);
+        unsigned mask = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mask |= (e & 1 ? v[e / 2].y : v[e / 2].x) >= bound ? 1u << e : 0u;
+        for (;;) {  // a value of every lane that has one
+          const unsigned votes = __ballot_sync(kAll, mask != 0);
+          if (votes == 0) break;
+          unsigned pos = 0;
+          if (lane == 0) pos = atomicAdd(&work.listed, (unsigned)__popc(votes));
+          pos = __shfl_sync(kAll, pos, 0) + __popc(votes & ((1u << lane) - 1u));
+          if (mask != 0 && pos < kList) {
+            const int col = sl.head + vec[s] * E + __ffs(mask) - 1;
+            work.list[pos] = entryOf(toFloat(sl.row[col]), col);
+          }
+          mask &= mask - 1;
+        }
       }
     }
-  }
   const int loose = tid < 2 * E ? sl.looseCol(tid) : -1;
   if (loose >= 0) {
     const float v = toFloat(sl.row[loose]);
