@@ -297,23 +297,30 @@ __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
   constexpr int U = kBatch;
   constexpr uint32_t w = Vec<T>::kMinusInf;
   const uint4* vecs = reinterpret_cast<const uint4*>(sl.row + sl.head);
-  uint4 raw[U];
-  auto fetch = [&](int i) {
+  const int whole = (sl.v1 - sl.v0) / (U * kWidth), left = sl.v1 - sl.v0 - whole * (U * kWidth);
+  int i = sl.v0 + (int)threadIdx.x % kWidth;
+  uint4 raw[U], now[U];
+  auto fetch = [&](int b) {
+    if (b < whole) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      raw[u] = i + u * kWidth < sl.v1 ? __ldg(vecs + i + u * kWidth) : make_uint4(w, w, w, w);
+      for (int u = 0; u < U; ++u) raw[u] = __ldg(vecs + i + u * kWidth);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        raw[u] = i + u * kWidth < sl.v1 ? __ldg(vecs + i + u * kWidth) : make_uint4(w, w, w, w);
+    }
   };
   ThreadSums acc(c);
-  const int batches = (sl.v1 - sl.v0 + U * kWidth - 1) / (U * kWidth);
-  int i = sl.v0 + (int)threadIdx.x % kWidth;
-  fetch(i);
-  for (int b = 0; b < batches; ++b, i += U * kWidth) {
-    uint4 now[U];
+  if (whole > 0 || left > 0) fetch(0);
+  for (int b = 0; b < whole; ++b) {
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = raw[u];
-    fetch(i + U * kWidth);
-    acc.add<T, kEntropy, false>(now, hook.batch(now, b == 0, i, sl), (sl.v1 - (i - (int)(threadIdx.x & 31)) + kWidth - 1) / kWidth, c);
+    i += U * kWidth;
+    if (b + 1 < whole || left > 0) fetch(b + 1);
+    acc.add<T, kEntropy, true>(now, hook.batch(now, b == 0, i - U * kWidth, sl), U, c);
   }
+  if (left > 0)
+    acc.add<T, kEntropy, false>(raw, hook.batch(raw, whole == 0, i, sl), (sl.v1 - (i - (int)(threadIdx.x & 31)) + kWidth - 1) / kWidth, c);
   return acc.sums();
 }
 

@@ -368,7 +368,7 @@ struct TopSlices {
 
 // Few rows: one per cluster.
 template <typename T, bool kEntropy, bool kTop>
-__global__ void __launch_bounds__(kThreads, kTop ? 3 : 4)
+__global__ void __launch_bounds__(kThreads, kTop ? 5 : 4)
 token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) unsigned char dynamic[];
