@@ -630,7 +630,7 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArg
                        loss, stats, pairs);
   const int words = kRest ? Marks<T>::words(x.vocab / Vec<T>::kElems) : 0;
   const size_t stay = sizeof(DistillRows) + (kRest ? 2 * (size_t)words : kNameWords) * 4;
-  // Two blocks of the form that stays have to fit on a multiprocessor; up to 65536 tokens of 16 bits three do.
+  // Two blocks of the form that stays have to fit on a multiprocessor; with up to 57344 tokens of 16 bits three do.
   if (manyRows(x.rows, sm_count) && stay <= 112 * 1024) {
     const int rows_a_block = rowsABlock(x, sizeof(T), sm_count);
     return launchRows(distillation_rows_kernel<T, kRest>, x.rows, rows_a_block, stay, stream, logits, x, given, c, inv_t, loss, stats,
@@ -638,11 +638,8 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArg
   }
   const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
   const size_t shared = 4 * (kNameWords + (kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) : 0));
-  if (shared > 32 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(distillation_slices_kernel<T, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)shared);
-    if (e != cudaSuccess) return e;
-  }
+  if (shared > 32 * 1024)
+    cudaFuncSetAttribute(distillation_slices_kernel<T, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
   return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, shared, stream, logits, x, given, c, inv_t, loss,
                       stats, pairs);
 }

@@ -141,18 +141,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return unpacked(r);
 }
 
-// Threads that finish a row together: all of a block, or some warps of it under a barrier of their own.
-struct BlockGroup {
-  static constexpr int kSize = kThreads;
-  static __device__ __forceinline__ int rank() { return threadIdx.x; }
-  static __device__ __forceinline__ void sync() { __syncthreads(); }
-};
-template <int kFirst, int kCount, int kBarrier> struct PartGroup {
-  static constexpr int kSize = kCount;
-  static __device__ __forceinline__ int rank() { return (int)threadIdx.x - kFirst; }
-  static __device__ __forceinline__ void sync() { asm volatile("bar.sync %0, %1;" ::"n"(kBarrier), "n"(kCount) : "memory"); }
-};
-
 template <typename T> __device__ __forceinline__ T* rowOf(const LogitRows& x, T* data, int64_t r) {
   const int64_t outer = x.inner == x.rows ? 0 : r / x.inner;
   return data + outer * x.outer_stride + (r - outer * x.inner) * x.row_stride;
@@ -442,9 +430,9 @@ cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, si
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
   config.numAttrs = slices > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, Params(args)...);
+  cudaLaunchKernelEx(&config, kernel, Params(args)...);
   noteLocalLaunch();
-  return e;
+  return cudaGetLastError();
 }
 
 // ---- many rows -----------------------------------------------------------------
@@ -721,8 +709,7 @@ template <class Finish> __device__ __forceinline__ void finishRows(HandOver& out
 
 template <typename... Params, typename... Args>
 cudaError_t launchRows(void (*kernel)(Params...), int64_t rows, int rows_a_block, size_t shared, cudaStream_t stream, Args... args) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-  if (e != cudaSuccess) return e;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
   kernel<<<(unsigned)((rows + rows_a_block - 1) / rows_a_block), kRowThreads, shared, stream>>>(Params(args)...);
   noteLocalLaunch();
   return cudaGetLastError();

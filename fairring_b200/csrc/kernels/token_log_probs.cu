@@ -43,28 +43,17 @@ struct TopWork {
   unsigned queued, listed, digit, left;
 };
 
-// Falling (or rising) order of 32 values, one per lane.
-__device__ __forceinline__ float sortedLanes(float v, bool falling) {
+// Falling order of 32 values, one per lane.
+__device__ __forceinline__ float sortedLanes(float v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
     for (int step = size / 2; step > 0; step /= 2) {
       const float o = __shfl_xor_sync(kAll, v, step);
-      const bool larger = ((lane & step) == 0) == ((size == 32 || (lane & size) == 0) == falling);
+      const bool larger = ((lane & step) == 0) == (size == 32 || (lane & size) == 0);
       v = larger ? fmaxf(v, o) : fminf(v, o);
     }
-  return v;
-}
-// Falling order of the 32 largest of 64 values, two per lane.
-__device__ __forceinline__ float sortedLanes(float a, float b) {
-  float v = fmaxf(sortedLanes(a, true), sortedLanes(b, false));
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int step = 16; step > 0; step /= 2) {
-    const float o = __shfl_xor_sync(kAll, v, step);
-    v = (lane & step) == 0 ? fmaxf(v, o) : fminf(v, o);
-  }
   return v;
 }
 
@@ -99,14 +88,14 @@ struct TopHook {
 };
 
 // The `want` largest of the first n entries of the list, in falling order, to `best`.
-template <class G> __device__ __forceinline__ void rankList(TopWork& work, int n, int want) {
+__device__ __forceinline__ void rankList(TopWork& work, int n, int want) {
   uint64_t* list = work.list;
-  if (n <= 2 * G::kSize) {  // every entry counts those above it, two threads an entry where there are threads enough
-    if (G::rank() == 0 && (n & 1)) list[n] = 0;
-    if (n & 1) G::sync();
-    const bool split = 2 * n <= G::kSize;
-    const int pairs = (n + 1) / 2, from = split && (G::rank() & 1) ? pairs / 2 : 0, to = split && !(G::rank() & 1) ? pairs / 2 : pairs;
-    for (int i = split ? G::rank() / 2 : G::rank(); i < (split ? G::kSize / 2 : (n + 31) / 32 * 32); i += G::kSize) {
+  if (n <= 2 * kThreads) {  // every entry counts those above it, two threads an entry where there are threads enough
+    if ((int)threadIdx.x == 0 && (n & 1)) list[n] = 0;
+    if (n & 1) __syncthreads();
+    const bool split = 2 * n <= kThreads;
+    const int pairs = (n + 1) / 2, from = split && ((int)threadIdx.x & 1) ? pairs / 2 : 0, to = split && !((int)threadIdx.x & 1) ? pairs / 2 : pairs;
+    for (int i = split ? (int)threadIdx.x / 2 : (int)threadIdx.x; i < (split ? kThreads / 2 : (n + 31) / 32 * 32); i += kThreads) {
       const uint64_t mine = i < n ? list[i] : 0;
       int above = 0;
 #pragma unroll 4
@@ -118,40 +107,40 @@ template <class G> __device__ __forceinline__ void rankList(TopWork& work, int n
       if (split) above += __shfl_xor_sync(kAll, above, 1);
       if (i < n && above < want) work.best[above] = mine;
     }
-    G::sync();
+    __syncthreads();
     return;
   }
   int size = 2;
   while (size < n) size *= 2;
-  for (int i = n + G::rank(); i < size; i += G::kSize) list[i] = 0;
-  G::sync();
+  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) list[i] = 0;
+  __syncthreads();
   for (int block = 2; block <= size; block *= 2)
     for (int step = block / 2; step > 0; step /= 2) {
-      for (int i = G::rank(); i < size / 2; i += G::kSize) {
+      for (int i = (int)threadIdx.x; i < size / 2; i += kThreads) {
         const int a = 2 * i - (i & (step - 1)), b = a + step;
         const uint64_t x = list[a], y = list[b];
         if ((x < y) == ((a & block) == 0)) list[a] = y, list[b] = x;
       }
-      G::sync();
+      __syncthreads();
     }
-  for (int i = G::rank(); i < want; i += G::kSize) work.best[i] = list[i];
-  G::sync();
+  for (int i = (int)threadIdx.x; i < want; i += kThreads) work.best[i] = list[i];
+  __syncthreads();
 }
 
 // The `want` largest of the slice's entries, to the list in any order, by a radix select that reads the slice six
 // times and more: for rows where the bound lets too much pass (ties, rising logits) and those with NaN.
-template <class G, typename T> __device__ __noinline__ void selectExactly(const Slice<T>& sl, int want, TopWork& work) {
-  const int tid = G::rank(), lane = threadIdx.x & 31;
+template <typename T> __device__ __noinline__ void selectExactly(const Slice<T>& sl, int want, TopWork& work) {
+  const int tid = threadIdx.x, lane = threadIdx.x & 31;
   uint32_t prefix = 0;
   unsigned left = want;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += G::kSize) work.hist[i] = 0;
-    G::sync();
-    for (int col = sl.c0 + tid; col < sl.c1; col += G::kSize) {
+    for (int i = tid; i < 256; i += kThreads) work.hist[i] = 0;
+    __syncthreads();
+    for (int col = sl.c0 + tid; col < sl.c1; col += kThreads) {
       const uint32_t key = keyOf(toFloat(sl.row[col]));
       if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&work.hist[key >> shift & 255u], 1u);
     }
-    G::sync();
+    __syncthreads();
     if (tid == 0) {
       int digit = 255;
       unsigned more = left;
@@ -159,74 +148,68 @@ template <class G, typename T> __device__ __noinline__ void selectExactly(const 
       work.digit = digit;
       work.left = more;
     }
-    G::sync();
+    __syncthreads();
     prefix = prefix << 8 | work.digit;
     left = work.left;
-    G::sync();
+    __syncthreads();
   }
   // `prefix` is the key of the last one; `left` of those that equal it are taken, the first ones.
   if (tid == 0) work.listed = 0;
-  G::sync();
-  for (int col = sl.c0 + tid; col < sl.c1; col += G::kSize) {
+  __syncthreads();
+  for (int col = sl.c0 + tid; col < sl.c1; col += kThreads) {
     const float v = toFloat(sl.row[col]);
     if (keyOf(v) > prefix) work.list[atomicAdd(&work.listed, 1u)] = entryOf(v, col);
   }
   const unsigned larger = want - left;
   unsigned taken = 0;
-  for (int base = sl.c0; base < sl.c1 && taken < left; base += G::kSize) {
+  for (int base = sl.c0; base < sl.c1 && taken < left; base += kThreads) {
     const int col = base + tid;
     const float v = col < sl.c1 ? toFloat(sl.row[col]) : 0.f;
     const bool equal = col < sl.c1 && keyOf(v) == prefix;
     const unsigned votes = __ballot_sync(kAll, equal);
-    G::sync();
+    __syncthreads();
     if (lane == 0) work.hist[tid >> 5] = __popc(votes);
-    G::sync();
+    __syncthreads();
     unsigned before = taken + __popc(votes & ((1u << lane) - 1u)), all = 0;
-    for (int w = 0; w < G::kSize / 32; ++w) {
+    for (int w = 0; w < kThreads / 32; ++w) {
       if (w < tid >> 5) before += work.hist[w];
       all += work.hist[w];
     }
     if (equal && before < left) work.list[larger + before] = entryOf(v, col);
     taken += all;
   }
-  G::sync();
+  __syncthreads();
 }
 
 // The slice's largest entries, at most k, in falling order, to `best`, zeros behind them up to k.  The sweep is over for all of the
-// group, and work.queued and work.listed are 0; they are 0 again afterwards.
+// block, and work.queued and work.listed are 0; they are 0 again afterwards.
 //
-// If each of the group's w warps finds r = ceil(k / w) values of `bound` or more among the largest values of the sweep's columns of
-// threads, k values of the slice are that large: each warp sorts what it has of those and gives its r-th, and the smallest
-// of these is the bound.  Groups below it are out, a hundred or two of the 2048 are looked into again, and what they have above the
-// bound, again a hundred or two values, is ranked.
-template <class G, typename T>
+// If each of the block's w warps finds r = ceil(k / w) values of `bound` or more among its threads' largest, k values of the slice
+// are that large: each warp sorts those of its threads and gives its r-th, and the smallest of these is the bound.  Groups below
+// it are out, a hundred or two of the 2048 are looked into again, and what they have above the bound, again a hundred or
+// two values, is ranked.
+template <typename T>
 __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, const Groups& groups, TopWork& work) {
-  constexpr int E = Vec<T>::kElems, kColumns = kThreads / G::kSize, kGroupWarps = G::kSize / 32;
-  static_assert(kColumns == 1 || kColumns == 2, "columns of threads that a thread looks at");
-  const int tid = G::rank(), lane = threadIdx.x & 31, want = min(k, sl.c1 - sl.c0);
+  constexpr int E = Vec<T>::kElems;
+  const int tid = threadIdx.x, lane = tid & 31, want = min(k, sl.c1 - sl.c0);
   const int batches = TopHook::batches(sl), span = TopHook::spanOf(sl), number = (batches + span - 1) / span;
-  float value[kGroups * kColumns], top[kColumns];
+  float value[kGroups], top = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < kColumns; ++j) {
-    top[j] = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      value[j * kGroups + g] = g < number ? groups.top[g][tid + j * G::kSize] : -INFINITY;
-      top[j] = fmaxf(top[j], value[j * kGroups + g]);
-    }
+  for (int g = 0; g < kGroups; ++g) {
+    value[g] = g < number ? groups.top[g][tid] : -INFINITY;
+    top = fmaxf(top, value[g]);
   }
-  const float sorted = kColumns == 1 ? sortedLanes(top[0], true) : sortedLanes(top[0], top[kColumns - 1]);
-  const float mine = __shfl_sync(kAll, sorted, (k + kGroupWarps - 1) / kGroupWarps - 1);
+  const float mine = __shfl_sync(kAll, sortedLanes(top), (k + kWarps - 1) / kWarps - 1);
   if (lane == 0) work.bound[tid >> 5] = mine;
-  G::sync();
+  __syncthreads();
   float bound = work.bound[0];
 #pragma unroll
-  for (int w = 1; w < kGroupWarps; ++w) bound = fminf(bound, work.bound[w]);
+  for (int w = 1; w < kWarps; ++w) bound = fminf(bound, work.bound[w]);
   bound = fmaxf(bound, -FLT_MAX);  // minus infinity is left to the other way
   // A thread's groups side by side in the queue, those of a warp after one addition to its length.
   unsigned pass = 0;
 #pragma unroll
-  for (int j = 0; j < kColumns * kGroups; ++j) pass |= value[j] >= bound ? 1u << j : 0u;
+  for (int g = 0; g < kGroups; ++g) pass |= value[g] >= bound ? 1u << g : 0u;
   int pos = __popc(pass);
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
@@ -237,15 +220,14 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
   if (lane == 31) at = atomicAdd(&work.queued, (unsigned)pos);
   pos += __shfl_sync(kAll, at, 31) - __popc(pass);
   for (; pass != 0; pass &= pass - 1, ++pos) {
-    const int j = __ffs(pass) - 1;
-    if (pos < kQueue) work.queue[pos] = j % kGroups * kThreads + tid + j / kGroups * G::kSize;
+    if (pos < kQueue) work.queue[pos] = (__ffs(pass) - 1) * kThreads + tid;
   }
-  G::sync();
+  __syncthreads();
   const int queued = work.queued;
   const bool fits = queued <= kQueue;
   const uint4* all = reinterpret_cast<const uint4*>(sl.row + sl.head);
   // kBatch threads a group, one for each of the vectors that a batch has of it; two rounds of groups at once.
-  constexpr int kRound = G::kSize / kBatch, kAhead = 2;
+  constexpr int kRound = kThreads / kBatch, kAhead = 2;
   for (int first = 0; first < queued && fits; first += kAhead * kRound)
     for (int batch = 0; batch < span; ++batch) {
       uint4 raw[kAhead];
@@ -289,16 +271,16 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
     const unsigned pos = v >= bound ? atomicAdd(&work.listed, 1u) : kList;
     if (pos < kList) work.list[pos] = entryOf(v, loose);
   }
-  G::sync();
+  __syncthreads();
   int n = work.listed;
-  G::sync();
+  __syncthreads();
   if (nan || !fits || n > kList || n < want) {
-    if (want > 0) selectExactly<G>(sl, want, work);
+    if (want > 0) selectExactly(sl, want, work);
     n = want;
   }
   if (tid == 0) work.listed = work.queued = 0;
-  for (int i = want + tid; i < k; i += G::kSize) work.best[i] = 0;
-  rankList<G>(work, n, want);
+  for (int i = want + tid; i < k; i += kThreads) work.best[i] = 0;
+  rankList(work, n, want);
 }
 
 // The k largest of the row from the slices' results, in block 0.  clusterSums() has waited for those.
@@ -312,7 +294,7 @@ __device__ __forceinline__ void clusterTop(int k, TopWork& work) {
     work.list[i] = cluster.map_shared_rank(&work, r)->best[i - r * k];
   }
   __syncthreads();
-  rankList<BlockGroup>(work, slices * k, k);
+  rankList(work, slices * k, k);
 }
 
 // What one row leaves; any pointer but `tokens` may be null.  Kept for the backward: m and S as its exponents need it, which is
@@ -350,10 +332,10 @@ struct Outputs {
     if (kEntropy) entropy[r] = low - acc.a / acc.s * kLn2;
     if (stats != nullptr) stats[r] = make_float2(acc.m, known ? acc.s * exp2Of(Exponent::excess(acc.m, c)) : nan);
   }
-  template <class G>
+  // By a block.
   __device__ __forceinline__ void largest(int64_t r, const Sums& acc, const uint64_t* best, float inv_t) const {
     const float low = logf(acc.s);
-    for (int i = G::rank(); i < k; i += G::kSize) {
+    for (int i = (int)threadIdx.x; i < k; i += kThreads) {
       const uint64_t entry = best[i];
       top_log_probs[r * k + i] = fmaf(valueOf((uint32_t)(entry >> 32)) - acc.m, inv_t, -low);
       top_tokens[r * k + i] = (int)~(uint32_t)entry;
@@ -402,7 +384,7 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
     if (col >= 0) acc.add<kEntropy>(toFloat(sl.row[col]), c);
   }
   acc = blockSums<kEntropy>(acc, c, scratch);
-  if constexpr (kTop) sliceTop<BlockGroup>(sl, out.k, acc.s != acc.s, top->groups, top->work);
+  if constexpr (kTop) sliceTop(sl, out.k, acc.s != acc.s, top->groups, top->work);
   if (slices > 1) {
     acc = clusterSums<kEntropy>(acc, c, &mine);
     if constexpr (kTop) clusterTop(out.k, top->work);
@@ -411,7 +393,7 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
   }
   if (!acc.template settle<kEntropy>(c)) acc = blockAgain<T, kEntropy>(sl.row, x.vocab, c, scratch, LeaveNone());
   if (threadIdx.x == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
-  if constexpr (kTop) out.largest<BlockGroup>(r, acc, top->work.best, inv_t);
+  if constexpr (kTop) out.largest(r, acc, top->work.best, inv_t);
 }
 
 // Many short rows: one per warp.
@@ -482,7 +464,7 @@ token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs o
 
 // A block does one batch of vectors of one row, so that all blocks are alike whatever the vocabulary.
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kEntropy ? 6 : 1)
 token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restrict__ grad,
                            const int64_t* __restrict__ tokens, const float2* __restrict__ stats,
                            const float* __restrict__ entropy, const float* __restrict__ g_log_probs, int64_t g_stride,

@@ -53,9 +53,12 @@ def _check(logits, tokens, temperature=1.0, entropy=True):
     p = logp.exp()
     size = p * (g.double().abs().unsqueeze(-1) + (h.double().abs() * (1 + want_h)).unsqueeze(-1) * (1 + logp.clamp_min(-110).abs())) / temperature
     room = half_step(logits.dtype) * want_grad.abs() + 2 * relative(logp) * size + smallest_step(logits.dtype)
+    # A probability below 2^-126 is zero, and its entry then off by as much times the factor: with one over T it may be a normal number.
+    room = room + 2.0 ** -126 * (g.double().abs() + 128 * h.double().abs()).unsqueeze(-1) / temperature
     room = room + 2.0 ** -22 * g.double().abs().unsqueeze(-1) / temperature * torch.zeros_like(p).scatter_(
         -1, tokens.clamp_min(0).unsqueeze(-1), 1.0)
-    bad = (grad.double() - want_grad).abs() > room
+    beyond = (want_grad.abs() > torch.finfo(logits.dtype).max) & (grad == want_grad.sign() * float("inf"))  # as it rounds
+    bad = ((grad.double() - want_grad).abs() > room) & ~beyond
     assert not bad.any(), (int(bad.sum()), float((grad.double() - want_grad).abs().max()))
     return got, grad
 
@@ -81,6 +84,24 @@ def test_every_row_length(rows, vocab, dtype):
 def test_temperature(temperature, entropy, dtype):
     logits = _logits(37, 5003, dtype)
     _check(logits, torch.randint(0, 5003, (37,), device="cuda", generator=_gen(2)), temperature, entropy)
+
+
+# few rows, a row per warp, blocks that stay
+@pytest.mark.parametrize("rows,vocab", [(5, 20011), (700, 1003), (700, 9001)])
+@pytest.mark.parametrize("entropy", [False, True])
+def test_where_the_fast_exponent_does_not_reach(rows, vocab, entropy):
+    """Logits far from zero, temperatures near zero and far above one, and all of them in one batch."""
+    for dtype in DTYPES:
+        tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(9))
+        logits = _logits(rows, vocab, dtype)
+        tokens[::3] = logits[::3].float().argmax(-1)
+        for temperature in (1e-6, 1e-3, 1e6):
+            _check(logits, tokens, temperature, entropy)
+    logits = _logits(rows, vocab, torch.float32)
+    for shift in (3e6, -3e6, 1e30, -1e30):
+        part = logits.clone()
+        part[::2] += shift
+        _check(part, tokens, 1.0, entropy)
 
 
 @pytest.mark.parametrize("rows,vocab", [(3, 1001), (3, 50265), (300, 20000), (1301, 1001), (1301, 20000)])
