@@ -493,8 +493,7 @@ struct Place {
   }
 };
 
-// The rows that a block has taken.  Whoever gives up a wait has the block stop; what it has taken and not finished is NaN, which the
-// fetching warp writes before it hands a row on.
+// The rows that a block has taken.  Whoever gives up a wait has the block stop; what it has taken and not finished is NaN.
 struct HandOver {
   alignas(16) uint4 answer;
   uint64_t answered;
@@ -533,9 +532,13 @@ struct HandOver {
                  "r"(sharedAddress(&answered))
                  : "memory");
   }
-  // By a warp: the number of the block that will not start, or -1 if all have.
+  // By a warp: the number of the block that will not start, or -1 if all have.  Waits whoever has given up: the answer comes to this
+  // block's memory.
   __device__ __forceinline__ int answerOf(unsigned parity) {
-    if (!wait(&answered, parity)) return -1;
+    if (!barrierWait(&answered, parity)) {
+      *static_cast<volatile int*>(&failed) = 1;
+      return -1;
+    }
     int block;
     uint32_t ok;
     asm volatile(
@@ -572,11 +575,12 @@ inline int rowsABlock(const LogitRows& x, int elem_size, int sm_count) {
 
 // The fetching warp's part.  `counts(r)`, by one lane, says that a row does not count as far as that is seen at once, else skip(r), by
 // one lane too.  prepare(r, place), by all, says for the others whether they do; mark(r, place) comes once the row's copies may begin.
+// lose(r), by one lane, leaves NaN: of every row before it is handed on, and of those that a block which gives up has taken.
 // Copies run kDepth - 1 batches ahead, so as many rows: nothing that a row's copies wait for may itself wait for one of the
 // kSlots - 1 rows before it.
 static_assert(kSlots >= kDepth, "a row's copies begin while the row kDepth - 1 before it is swept");
-template <class Counts, class Skip, class Prepare, class Mark>
-__device__ __forceinline__ void fetchRows(Counts&& counts, int64_t rows, int rows_a_block, HandOver& out, Skip&& skip,
+template <class Counts, class Skip, class Lose, class Prepare, class Mark>
+__device__ __forceinline__ void fetchRows(Counts&& counts, int64_t rows, int rows_a_block, HandOver& out, Skip&& skip, Lose&& lose,
                                           Prepare&& prepare, Mark&& mark) {
   const int lane = threadIdx.x & 31;
   Place place;
@@ -586,18 +590,17 @@ __device__ __forceinline__ void fetchRows(Counts&& counts, int64_t rows, int row
     const int64_t first = (int64_t)block * rows_a_block, mine = first + lane;
     const bool some = lane < rows_a_block && mine < rows, yes = some && counts((int)mine);
     if (some && !yes) skip((int)mine);
-    for (unsigned mask = __ballot_sync(kAll, yes); mask != 0; mask &= mask - 1) {
+    unsigned mask = __ballot_sync(kAll, yes);
+    for (; mask != 0; mask &= mask - 1) {
       const int r = (int)first + __ffs(mask) - 1;
-      if (!out.wait(&out.empty[place.slot], place.parity ^ 1)) {
-        barrierWait(&out.answered, parity);  // the answer is on its way to this block's memory
-        return;
-      }
+      if (!__all_sync(kAll, out.wait(&out.empty[place.slot], place.parity ^ 1))) break;
       if (!prepare(r, place)) {
         if (lane == 0) skip(r);
         continue;
       }
       __syncwarp();
       if (lane == 0) {
+        lose(r);
         out.row[place.slot] = r;
         barrierArrive(&out.ready[place.slot]);
       }
@@ -607,6 +610,12 @@ __device__ __forceinline__ void fetchRows(Counts&& counts, int64_t rows, int row
       place.next();
     }
     block = out.answerOf(parity);
+    if (__any_sync(kAll, out.gaveUp())) {
+      if (mask >> lane & 1u) lose((int)mine);
+      const int64_t next = (int64_t)block * rows_a_block + lane;
+      if (block >= 0 && lane < rows_a_block && next < rows) lose((int)next);
+      return;
+    }
   }
   if (!out.wait(&out.empty[place.slot], place.parity ^ 1)) return;
   if (lane == 0) {
