@@ -465,10 +465,12 @@ distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Given given,
     int fetched = 0, marked = -1, marked_before = -1;  // the rows whose listed tokens are marked
     fetchRows(
         [](int) { return true; }, x.rows, rows_a_block, hand, [&](int r) { skipRow(loss + r, stats + r); },
+        [&](int r) {
+          const float nan = __int_as_float(0x7fffffff);
+          loss[r] = nan, stats[r] = make_float4(nan, nan, nan, nan);
+        },
         [&](int r, const Place& at) {
           if (!countsAtAll<kRest>(given, r)) return false;
-          const float nan = __int_as_float(0x7fffffff);
-          if (lane == 0) loss[r] = nan, stats[r] = make_float4(nan, nan, nan, nan);  // stays if nobody comes to finish the row
           // The marks are waited for, so what can be done before the row is handed on is.
           if (kRest) loadTeacher<T, kRest>(shared.teacher[at.slot], given, r, rowOf(x, logits, r), x.vocab, (float)inv_t);
           return true;
@@ -539,6 +541,7 @@ distillation_mean_kernel(const float* __restrict__ loss, const float4* __restric
                          float* __restrict__ mean, float* __restrict__ count) {
   __shared__ double sums[32], numbers[32];
   double s = 0, n = 0;
+#pragma unroll 8
   for (int64_t r = threadIdx.x; r < rows; r += 1024) {
     s += loss[r];
     n += stats[r].w < 0.f ? 0 : 1;
@@ -674,7 +677,7 @@ cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const
 cudaError_t launchDistillation(const void* logits, const LogitRows& x, const DistillationArgs& a, float* loss, float* stats,
                                void* pairs, int sm_count, cudaStream_t stream) {
   if (x.rows <= 0) return cudaSuccess;
-  if (x.vocab <= 0 || x.rows > INT32_MAX || a.k <= 0 || a.k > kMostTeacherTokens || (a.rest && x.vocab > kMostRestVocab))
+  if (x.vocab <= 0 || x.vocab > kMostVocab || x.rows > INT32_MAX || a.k <= 0 || a.k > kMostTeacherTokens || (a.rest && x.vocab > kMostRestVocab))
     return cudaErrorInvalidValue;
   switch (x.type) {
     case LogitType::kBFloat16: return forwardOf<__nv_bfloat16>(logits, x, a, loss, stats, pairs, sm_count, stream);
@@ -694,7 +697,7 @@ cudaError_t launchDistillationBackward(const void* logits, const LogitRows& x, v
                                        const void* pairs, int k, double temperature, const float* upstream, int64_t stride,
                                        const float* count, cudaStream_t stream) {
   if (x.rows <= 0) return cudaSuccess;
-  if (x.vocab <= 0 || x.rows > INT32_MAX || k <= 0 || k > kMostTeacherTokens) return cudaErrorInvalidValue;
+  if (x.vocab <= 0 || x.vocab > kMostVocab || x.rows > INT32_MAX || k <= 0 || k > kMostTeacherTokens) return cudaErrorInvalidValue;
   // A vector of the logits becomes a vector of the gradient.
   if ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad)) & 15u) return cudaErrorMisalignedAddress;
   switch (x.type) {

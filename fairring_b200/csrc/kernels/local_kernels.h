@@ -140,6 +140,7 @@ cudaError_t launchStemFold(const void* image, bool bf16, void* out, int images, 
 
 // Rows of `vocab` logits in two levels of strides, in elements: row r starts at
 // (r / inner) * outer_stride + (r % inner) * row_stride.
+constexpr int kMostVocab = INT32_MAX - 1024;  // a column's number and a block's step past it are ints
 enum class LogitType { kFloat, kBFloat16, kHalf };
 struct LogitRows {
   int64_t rows, inner, outer_stride, row_stride;
@@ -178,9 +179,9 @@ struct TokenLogProbsGrads {
 cudaError_t launchTokenLogProbsBackward(const void* logits, const LogitRows& x, void* grad, const TokenLogProbsGrads& a,
                                         cudaStream_t stream);
 
-// Divergence of the rows' softmax from a teacher's `k` log probabilities a row; a negative token is padding.  `rest`:
-// what they leave of the probability, if it is more than the rounding of fp32 log probabilities, is one more class.  `stats` (4 floats a row) and `pairs` (k of token and
-// probability a row) are for the backward; `pairs` may be null.
+// Divergence of the rows' softmax from a teacher's `k` log probabilities a row; a negative token is padding.  `rest`: what
+// they leave of the probability, from kLeastRest on, is one more class.  `stats` (4 floats a row) and `pairs` (k of token
+// and probability a row) are for the backward; `pairs` may be null.
 constexpr int kMostTeacherTokens = 256;
 constexpr int kMostRestVocab = 1 << 20;
 constexpr double kLeastRest = 1.0 / (1 << 20);

@@ -443,11 +443,7 @@ token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs o
   if (threadIdx.x < kThreads + 32) {
     fetchRows(
         [&](int r) { return tokens == nullptr || tokens[r] >= 0; }, x.rows, rows_a_block, hand, [&](int r) { out.skipped(r); },
-        [&](int r, const Place&) {
-          if (lane == 0) out.broken(r);
-          return true;
-        },
-        [](int, const Place&) {});
+        [&](int r) { out.broken(r); }, [](int, const Place&) { return true; }, [](int, const Place&) {});
     return;
   }
   finishRows(hand, [&](int r, const Place& at) {
@@ -576,7 +572,7 @@ cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const
 cudaError_t launchTokenLogProbs(const void* logits, const LogitRows& x, const TokenLogProbsArgs& a, int sm_count,
                                 cudaStream_t stream) {
   if (x.rows <= 0) return cudaSuccess;
-  if (x.vocab <= 0 || x.rows > INT32_MAX || a.k < 0 || a.k > kMostTop || a.k > x.vocab) return cudaErrorInvalidValue;
+  if (x.vocab <= 0 || x.vocab > kMostVocab || x.rows > INT32_MAX || a.k < 0 || a.k > kMostTop || a.k > x.vocab) return cudaErrorInvalidValue;
   switch (x.type) {
     case LogitType::kBFloat16: return forwardOf<__nv_bfloat16>(logits, x, a, sm_count, stream);
     case LogitType::kHalf: return forwardOf<__half>(logits, x, a, sm_count, stream);
@@ -587,7 +583,7 @@ cudaError_t launchTokenLogProbs(const void* logits, const LogitRows& x, const To
 cudaError_t launchTokenLogProbsBackward(const void* logits, const LogitRows& x, void* grad, const TokenLogProbsGrads& a,
                                         cudaStream_t stream) {
   if (x.rows <= 0) return cudaSuccess;
-  if (x.vocab <= 0 || x.rows > INT32_MAX) return cudaErrorInvalidValue;
+  if (x.vocab <= 0 || x.vocab > kMostVocab || x.rows > INT32_MAX) return cudaErrorInvalidValue;
   // A vector of the logits becomes a vector of the gradient.
   if ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(grad)) & 15u) return cudaErrorMisalignedAddress;
   switch (x.type) {

@@ -25,7 +25,8 @@ void checkLogits(const at::Tensor& logits) {
   TORCH_CHECK_VALUE(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 ||
                         logits.scalar_type() == at::kHalf,
                     "logits must be fp32, bf16 or fp16");
-  TORCH_CHECK_VALUE(logits.size(-1) > 0 && logits.size(-1) <= INT32_MAX - 64, "the vocabulary must not be empty");
+  TORCH_CHECK_VALUE(logits.size(-1) > 0 && logits.size(-1) <= kMostVocab, "logits must have from 1 to ", kMostVocab,
+                    " columns, not ", logits.size(-1));
   TORCH_CHECK_VALUE(logits.numel() / logits.size(-1) <= INT32_MAX, "too many rows");
 }
 
@@ -152,9 +153,13 @@ TokenLogProbs tokenLogProbsForward(const Rows& rows, const std::optional<at::Ten
 // The gradient of the logits from torch's ops, where its own graph is wanted.
 at::Tensor tokenLogProbsBackwardGraph(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
                                       const at::Tensor& g_log_probs, const at::Tensor& g_entropy) {
-  const at::Tensor logp = at::log_softmax(logits.to(at::kFloat) / temperature, -1), p = logp.exp();
-  at::Tensor grad = at::zeros_like(p), counts;
-  if (tokens.defined()) counts = tokens.ge(0).unsqueeze(-1);
+  at::Tensor counts, wide = logits.to(at::kFloat);
+  if (tokens.defined()) {  // a row that does not count is not looked at, be it NaN
+    counts = tokens.ge(0).unsqueeze(-1);
+    wide = wide.masked_fill(counts.logical_not(), 0.0);
+  }
+  const at::Tensor logp = at::log_softmax(wide / temperature, -1), p = logp.exp();
+  at::Tensor grad = at::zeros_like(p);
   if (g_log_probs.defined()) {
     const at::Tensor known = tokens.ge(0).logical_and(tokens.lt(logits.size(-1))).unsqueeze(-1);
     const at::Tensor at = tokens.unsqueeze(-1).where(known, at::zeros_like(tokens).unsqueeze(-1));
@@ -296,14 +301,14 @@ Distillation distillationForward(const Rows& rows, const at::Tensor& tokens, con
 // The gradient of the logits from torch's ops, where its own graph is wanted.
 at::Tensor distillationBackwardGraph(const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& log_probs,
                                      double temperature, bool rest, bool mean, const at::Tensor& g, const at::Tensor& kept) {
-  const at::Tensor z = logits.to(at::kFloat) / temperature;
   const at::Tensor there = tokens.ge(0), bad = tokens.ge(logits.size(-1)).any(-1, true);
   const at::Tensor known = there.logical_and(tokens.lt(logits.size(-1)));
   const double low = -std::numeric_limits<double>::infinity();
   const at::Tensor at = tokens.where(known, at::zeros_like(tokens));
-  at::Tensor grad = at::softmax(z, -1), counts, q;
+  const at::Tensor counts = (rest ? there : there.logical_and(log_probs.eq(low).logical_not())).any(-1, true);
+  const at::Tensor z = logits.to(at::kFloat).masked_fill(counts.logical_not(), 0.0) / temperature;
+  at::Tensor grad = at::softmax(z, -1), q;
   if (rest) {
-    counts = there.any(-1, true);
     q = at::where(known, log_probs.exp(), at::zeros_like(log_probs));
     const at::Tensor mass = q.to(at::kDouble).sum(-1, true), some = 1 - mass;
     const at::Tensor left = at::where(some.ge(kLeastRest), some, at::zeros_like(some));
@@ -311,7 +316,6 @@ at::Tensor distillationBackwardGraph(const at::Tensor& logits, const at::Tensor&
     const at::Tensor share = at::softmax(z.masked_fill(listed, low), -1).masked_fill(listed, 0.0);
     grad = grad * (mass + left).to(at::kFloat) - at::where(left.gt(0), share * left.to(at::kFloat), at::zeros_like(share));
   } else {
-    counts = there.logical_and(log_probs.eq(low).logical_not()).any(-1, true);
     q = at::softmax((log_probs / temperature).masked_fill(known.logical_not(), low), -1).masked_fill(known.logical_not(), 0.0);
   }
   grad = grad.scatter_add(-1, at, -q);
@@ -384,6 +388,7 @@ void bindLogitsOps(pybind11::module_& m) {
         py::arg("entropy"), py::arg("top_k"));
   m.def("distillation", &distillation, py::arg("logits"), py::arg("tokens"), py::arg("log_probs"), py::arg("temperature"),
         py::arg("rest"), py::arg("mean"));
+  m.attr("MOST_VOCAB") = kMostVocab;
   m.attr("MOST_TOP_TOKENS") = kMostTopTokens;
   m.attr("MOST_TEACHER_TOKENS") = kMostTeacherTokens;
   m.attr("MOST_REST_VOCAB") = kMostRestVocab;

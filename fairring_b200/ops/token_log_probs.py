@@ -44,7 +44,7 @@ def _check_tokens(tokens: torch.Tensor, logits: torch.Tensor, shape, name: str) 
 def _takes(logits: torch.Tensor) -> bool:
     """Whether the kernels may be handed the logits."""
     return (ordinary(logits) and logits.is_cuda and plain_calls() and logits.dtype in _TYPES and logits.dim() > 0
-            and 0 < logits.shape[-1] <= 2 ** 31 - 65 and logits.numel() < logits.shape[-1] * 2 ** 31
+            and 0 < logits.shape[-1] <= _C.MOST_VOCAB and logits.numel() < logits.shape[-1] * 2 ** 31
             and not (torch.is_inference_mode_enabled() and logits.requires_grad))
 
 

@@ -346,3 +346,55 @@ def test_a_teacher_and_its_student():
         assert abs(float(loss) - float(want.sum()) / n) <= 2.0 ** -16
         _check(logits.detach(), top.top_tokens, given, 2.0, rest)
         assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in student.parameters())
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_second_derivative_past_rows_that_do_not_count(rest):
+    """A padded row's logits may be anything, its first and second derivatives are 0."""
+    from fairring_b200.ops import distillation_loss
+
+    x, tokens, given = _case(4, 33, 6, torch.float32)
+    x[2] = float("nan")  # _case pads that row
+    leaf = x.requires_grad_(True)
+    loss = distillation_loss(leaf, tokens, given - 0.1, rest=rest)
+    (g,) = torch.autograd.grad(loss ** 2, leaf, create_graph=True)
+    (h,) = torch.autograd.grad((g ** 2).sum(), leaf)
+    for d in (g, h):
+        assert bool((d[2] == 0).all()) and bool((d[0] != 0).any()) and bool(d.isfinite().all())
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(60, 20011), (1300, 20011), (1300, 1003)])
+def test_two_streams_at_once(rows, vocab, rest):
+    from fairring_b200.ops import distillation_loss
+
+    inputs = [_case(rows, vocab, 20, torch.bfloat16, seed=i) for i in range(2)]
+
+    def call(i):
+        leaf = inputs[i][0].detach().requires_grad_(True)
+        loss = distillation_loss(leaf, *inputs[i][1:], rest=rest)
+        return loss.detach(), torch.autograd.grad(loss, leaf)[0]
+
+    want = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_the_mean_of_very_many_rows():
+    from fairring_b200.ops import distillation_loss
+
+    x, tokens, given = _case(300_007, 24, 4, torch.bfloat16)
+    each = distillation_loss(x, tokens, given, reduction="none").double()
+    want = each.sum() / int((tokens >= 0).any(-1).sum())
+    # summed in 64 bits and rounded once
+    assert abs(float(distillation_loss(x, tokens, given)) - float(want)) <= 2.0 ** -23 * float(want)

@@ -399,3 +399,53 @@ def test_streams_and_graphs(rows):
     for i in range(2):
         for a, b in zip(outs[i], call(i)):
             assert torch.equal(a, b)
+
+
+def test_second_derivative_past_rows_that_do_not_count():
+    """A padded row's logits may be anything, its first and second derivatives are 0."""
+    from fairring_b200.ops import token_log_probs
+
+    x = _logits(3, 17, torch.float32)
+    x[1] = float("nan")
+    leaf = x.requires_grad_(True)
+    o = token_log_probs(leaf, torch.tensor([1, -100, 5], device="cuda"), entropy=True)
+    (g,) = torch.autograd.grad((o.log_probs ** 2).sum() + o.entropy.sum(), leaf, create_graph=True)
+    (h,) = torch.autograd.grad((g ** 2).sum(), leaf)
+    for d in (g, h):
+        assert bool((d[1] == 0).all()) and bool((d[::2] != 0).any()) and bool(d.isfinite().all())
+
+
+@pytest.mark.parametrize("rows,vocab,top_k", [(60, 20011, 0), (1300, 20011, 0), (1300, 1003, 0), (700, 20011, 9)])
+def test_two_streams_at_once(rows, vocab, top_k):
+    from fairring_b200.ops import token_log_probs
+
+    inputs = [(_logits(rows, vocab, torch.bfloat16, seed=i), torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(i)))
+              for i in range(2)]
+
+    def call(i):
+        leaf = inputs[i][0].detach().requires_grad_(True)
+        o = token_log_probs(leaf, inputs[i][1], entropy=True, top_k=top_k)
+        return [v.detach() for v in o if v is not None] + list(torch.autograd.grad(o.log_probs.sum() + o.entropy.sum(), leaf))
+
+    want = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_a_vocabulary_past_the_kernels():
+    """More columns than an int may step over: refused by the kernels' entry without a look at the logits."""
+    from fairring_b200 import _C
+
+    x = torch.zeros(1, device="cuda").expand(1, _C.MOST_VOCAB + 1)
+    with pytest.raises(ValueError):
+        _C.token_log_probs(x, torch.zeros(1, dtype=torch.long, device="cuda"), 1.0, False, 0)
