@@ -171,6 +171,7 @@ __device__ __forceinline__ unsigned markListed(const Teacher& te, int k, const S
 // Whether a token is named more than once, by one warp.  Its bit is that of its number's end: where another token had set it, that
 // token is looked for among all.  `bits`: `words` of zeros, a power of two, as they are again afterwards.
 constexpr int kNameWords = 1024;
+static_assert(kMostTeacherTokens <= kThreads, "a thread an entry");
 __device__ __forceinline__ bool namedTwice(const Teacher& te, int k, unsigned* bits, int words) {
   const int lane = threadIdx.x & 31;
   bool twice = false;
@@ -271,14 +272,16 @@ __device__ __forceinline__ void skipRow(float* loss, float4* stats) {
   *stats = make_float4(0.f, 0.f, 0.f, -1.f);
 }
 
-// Few rows: one per cluster.
+// Few rows: one per cluster.  Eight warps sweep, and one of the first block reads the teacher meanwhile.
+constexpr int kSliceThreads = kThreads + 32;
 template <typename T, bool kRest>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kSliceThreads, 4)
 distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given given, float c, double inv_t,
                            float* __restrict__ loss, float4* __restrict__ stats, int2* __restrict__ pairs) {
   namespace cg = cooperative_groups;
   __shared__ Teacher te;
-  __shared__ Sums scratch[kWarps], mine;
+  __shared__ Sums scratch[kWarps + 1], mine;
+  __shared__ Listed listed;
   __shared__ unsigned loose;
   extern __shared__ __align__(16) unsigned names[];
   unsigned* bits = names + kNameWords;  // with the rest
@@ -288,24 +291,19 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given give
   const int tid = threadIdx.x, k = given.k;
   const T* row = rowOf(x, logits, r);
   const Slice<T> sl(row, x.vocab, rank, slices);
-  RestHook<kThreads> hook;
-  hook.bits = bits;
   if (tid == 0) loose = 0;
   if (rank == 0)
-    for (int i = tid; i < kNameWords; i += kThreads) names[i] = 0;
+    for (int i = tid; i < kNameWords; i += kSliceThreads) names[i] = 0;
   if constexpr (kRest)
-    for (int i = tid; i < Marks<T>::words(sl.v1 - sl.v0); i += kThreads) bits[i] = 0;
-  bool some = false;
-  for (int i = tid; i < k; i += kThreads)
-    some |= given.tokens[r * k + i] >= 0 && (kRest || !(given.log_probs[r * k + i] == -INFINITY));
-  if (!__syncthreads_or(some)) {
+    for (int i = tid; i < Marks<T>::words(sl.v1 - sl.v0); i += kSliceThreads) bits[i] = 0;
+  int64_t t = -1;  // this thread's entry: there are no more than kThreads
+  if (tid < k) t = given.tokens[r * k + tid];
+  if (!__syncthreads_or(t >= 0 && (kRest || !(given.log_probs[r * k + tid] == -INFINITY)))) {
     if (rank == 0 && tid == 0) skipRow(loss + r, stats + r);
     return;
   }
   if constexpr (kRest) {
-    for (int i = tid; i < k; i += kThreads) {
-      const int64_t t = given.tokens[r * k + i];
-      if (t < sl.c0 || t >= sl.c1) continue;
+    if (t >= sl.c0 && t < sl.c1) {
       if (Marks<T>::loose(sl, (int)t))
         atomicOr(&loose, Marks<T>::looseBit(sl, (int)t));
       else
@@ -313,23 +311,26 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given give
     }
     __syncthreads();
   }
-  Listed l = {};
-  if (rank == 0 && tid < 32) {
-    loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
-    if (kRest || pairs != nullptr)
-      mergeTeacher(te, k, namedTwice(te, k, names, kNameWords), pairs != nullptr ? pairs + r * k : nullptr);
-    l = listedOf<kRest>(te, k, c);
-  }
-  Sums acc;
-  if constexpr (kRest) {
-    acc = scan<T, false, kThreads>(sl, c, hook);
+  Sums acc = Sums::none(c);
+  if (tid >= kThreads) {
+    if (rank == 0) {
+      loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
+      if (kRest || pairs != nullptr)
+        mergeTeacher(te, k, namedTwice(te, k, names, kNameWords), pairs != nullptr ? pairs + r * k : nullptr);
+      const Listed l = listedOf<kRest>(te, k, c);
+      if (tid == kThreads) listed = l;  // blockSums() has all wait for that
+    }
   } else {
-    NoHook none;
-    acc = scan<T, false, kThreads>(sl, c, none);
-  }
-  if (tid < 2 * Vec<T>::kElems) {
-    const int col = sl.looseCol(tid);
-    if (col >= 0 && !(loose >> tid & 1u)) acc.add<false>(toFloat(row[col]), c);
+    if constexpr (kRest) {
+      RestHook<kThreads> hook;
+      hook.bits = bits;
+      acc = scan<T, false, kThreads>(sl, c, hook);
+    } else {
+      NoHook none;
+      acc = scan<T, false, kThreads>(sl, c, none);
+    }
+    const int col = tid < 2 * Vec<T>::kElems && !(loose >> tid & 1u) ? sl.looseCol(tid) : -1;
+    if (col >= 0) acc.add<false>(toFloat(row[col]), c);
   }
   acc = blockSums<false>(acc, c, scratch);
   if (slices > 1) {
@@ -343,7 +344,7 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given give
     else
       acc = blockAgain<T, false>(row, x.vocab, c, scratch, LeaveNone());
   }
-  if (tid == 0) finishRow<kRest>(l, acc, te.outside, c, inv_t, loss + r, stats + r);
+  if (tid == 0) finishRow<kRest>(listed, acc, te.outside, c, inv_t, loss + r, stats + r);
 }
 
 // Many short rows: one per warp.
@@ -643,7 +644,7 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArg
   const size_t shared = 4 * (kNameWords + (kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) : 0));
   if (shared > 32 * 1024)
     cudaFuncSetAttribute(distillation_slices_kernel<T, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-  return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, shared, stream, logits, x, given, c, inv_t, loss,
+  return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, kSliceThreads, shared, stream, logits, x, given, c, inv_t, loss,
                       stats, pairs);
 }
 

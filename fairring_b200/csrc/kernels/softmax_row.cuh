@@ -351,7 +351,8 @@ template <bool kEntropy> __device__ __forceinline__ Sums warpSums(Sums acc, floa
   return {m, warpSum(acc.s), kEntropy ? warpSum(acc.a) : 0.f};
 }
 
-// The block's sums from its threads', in every thread.  `scratch`: kWarps of them in shared memory.
+// The block's sums from those of its first kThreads threads, in every thread; what others bring is not added.  `scratch`: one of
+// them a warp, in shared memory.
 template <bool kEntropy> __device__ __forceinline__ Sums blockSums(Sums acc, float c, Sums* scratch) {
   acc = warpSums<kEntropy>(acc, c);
   __syncthreads();
@@ -363,15 +364,16 @@ template <bool kEntropy> __device__ __forceinline__ Sums blockSums(Sums acc, flo
   return acc;
 }
 
-// A row's sums, relative to m, by a whole block or a whole warp, where the sweep's did not settle.
+// A row's sums, relative to m, by a whole block, its first kThreads threads, or a whole warp, where the sweep's did not settle.
 template <typename T, bool kEntropy, class Leave>
 __device__ __noinline__ Sums blockAgain(const T* row, int vocab, float c, Sums* scratch, Leave leave) {
-  float top = warpMax(largestOf(row, vocab, (int)threadIdx.x, kThreads, leave));
+  const int mine = threadIdx.x < kThreads ? vocab : 0;
+  float top = warpMax(largestOf(row, mine, (int)threadIdx.x, kThreads, leave));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5].m = top;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) top = fmaxf(top, scratch[i].m);
-  Sums acc = lookAgain<T, kEntropy>(row, vocab, (int)threadIdx.x, kThreads, c, top, leave);
+  Sums acc = lookAgain<T, kEntropy>(row, mine, (int)threadIdx.x, kThreads, c, top, leave);
   acc.s = warpSum(acc.s);
   acc.a = warpSum(acc.a);
   __syncthreads();
@@ -417,11 +419,11 @@ inline int slicesFor(int64_t rows, int vocab, int elem_size, int sm_count) {
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, size_t shared, cudaStream_t stream,
+cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, int threads, size_t shared, cudaStream_t stream,
                          Args... args) {
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)(rows * slices));
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3((unsigned)threads);
   config.dynamicSmemBytes = shared;
   config.stream = stream;
   cudaLaunchAttribute attribute = {};

@@ -537,9 +537,9 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const Outputs& out, d
   }
   const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
   if (out.k > 0)
-    return launchSlices(token_log_probs_slices_kernel<T, kEntropy, true>, x.rows, slices,
+    return launchSlices(token_log_probs_slices_kernel<T, kEntropy, true>, x.rows, slices, kThreads,
                         sizeof(TopSlices), stream, logits, x, out, c, inv_t);
-  return launchSlices(token_log_probs_slices_kernel<T, kEntropy, false>, x.rows, slices, 0, stream, logits, x, out, c, inv_t);
+  return launchSlices(token_log_probs_slices_kernel<T, kEntropy, false>, x.rows, slices, kThreads, 0, stream, logits, x, out, c, inv_t);
 }
 
 template <typename T>
