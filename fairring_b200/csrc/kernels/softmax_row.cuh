@@ -409,12 +409,17 @@ template <bool kEntropy> __device__ __forceinline__ Sums clusterSums(Sums mine, 
 }
 __device__ __forceinline__ void clusterDone() { cooperative_groups::this_cluster().sync(); }
 
-// Into how many slices `rows` rows are cut, as a power of two: as many as keep two blocks a multiprocessor busy, but not
-// so many that a block's slice is less than half a batch.
+// Into how many slices `rows` rows are cut, as a power of two: as many as keep two blocks a multiprocessor busy, but not so many that a
+// block's slice is less than half a batch.  Three blocks where the slices stay long: 200 rows of 128003 fp32 logits with the rest
+// 38.8 us in one slice each and 29.6 in two, 100 rows 21.6 in two and 17.7 in four; but 48 rows of 51200 bf16 logits with 20 entries
+// 11.1 in four and 13.3 in eight, 200 rows of 8192 fp32 logits 5.6 in one and 6.5 in two.
+constexpr int kLongSlice = 56 * 1024;  // bytes
 inline int slicesFor(int64_t rows, int vocab, int elem_size, int sm_count) {
-  const int64_t vecs = (int64_t)vocab * elem_size / 16;
+  const int64_t bytes = (int64_t)vocab * elem_size;
   int n = 1;
-  while (n < kMostSlices && rows * n * 2 <= 2 * (int64_t)sm_count && vecs / (n * 2) >= kThreads * kBatch / 2) n *= 2;
+  while (n < kMostSlices && rows * n * 2 <= (bytes / (n * 2) >= kLongSlice ? 3 : 2) * (int64_t)sm_count &&
+         bytes / 16 / (n * 2) >= kThreads * kBatch / 2)
+    n *= 2;
   return n;
 }
 

@@ -184,8 +184,8 @@ template <typename T> __device__ __noinline__ void selectExactly(const Slice<T>&
 // The slice's largest entries, at most k, in falling order, to `best`, zeros behind them up to k.  The sweep is over for all of the
 // block, and work.queued and work.listed are 0; they are 0 again afterwards.
 //
-// If each of the block's w warps finds r = ceil(k / w) values of `bound` or more among its threads' largest, k values of the slice
-// are that large: each warp sorts those of its threads and gives its r-th, and the smallest of these is the bound.  Groups below
+// If each of w warps finds r = ceil(k / w) values of `bound` or more among its threads' largest, k values of the slice are that
+// large: each warp sorts those of its threads and gives its r-th, and the smallest of these is the bound.  Groups below
 // it are out, a hundred or two of the 2048 are looked into again, and what they have above the bound, again a hundred or
 // two values, is ranked.
 template <typename T>
@@ -199,12 +199,14 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
     value[g] = g < number ? groups.top[g][tid] : -INFINITY;
     top = fmaxf(top, value[g]);
   }
-  const float mine = __shfl_sync(kAll, sortedLanes(top), (k + kWarps - 1) / kWarps - 1);
-  if (lane == 0) work.bound[tid >> 5] = mine;
+  const int warps = min(kWarps, (sl.v1 - sl.v0) / 32), of_each = warps > 0 ? (k + warps - 1) / warps : k;  // warps that are all at work
+  const float mine = __shfl_sync(kAll, sortedLanes(top), (of_each - 1) & 31);
+  if (lane == 0) work.bound[tid >> 5] = tid >> 5 < warps ? mine : INFINITY;
   __syncthreads();
   float bound = work.bound[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) bound = fminf(bound, work.bound[w]);
+  if (of_each > 32) bound = -FLT_MAX;
   bound = fmaxf(bound, -FLT_MAX);  // minus infinity is left to the other way
   // A thread's groups side by side in the queue, those of a warp after one addition to its length.
   unsigned pass = 0;
