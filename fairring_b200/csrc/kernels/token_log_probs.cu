@@ -40,6 +40,7 @@ struct TopWork {
   unsigned hist[256];
   int queue[kQueue];
   float bound[kWarps];
+  unsigned above[kWarps];
   unsigned queued, listed, digit, left;
 };
 
@@ -182,11 +183,11 @@ template <typename T> __device__ __noinline__ void selectExactly(const Slice<T>&
 }
 
 // The slice's largest entries, at most k, in falling order, to `best`, zeros behind them up to k.  The sweep is over for all of the
-// block, and work.queued and work.listed are 0; they are 0 again afterwards.
+// block, and work.queued, work.listed and work.above are 0.
 //
-// If each of w warps finds r = ceil(k / w) values of `bound` or more among its threads' largest, k values of the slice are that
-// large: each warp sorts those of its threads and gives its r-th, and the smallest of these is the bound.  Groups below
-// it are out, a hundred or two of the 2048 are looked into again, and what they have above the bound, again a hundred or
+// If k of the threads' largest values are as large as `bound`, k values of the slice are.  Each of w warps sorts those of its threads
+// and gives its r-th, r = ceil(k / w): that many are as large as the smallest of these, and the largest of them that k values
+// reach is the bound.  Groups below it are out, a hundred or two of the 2048 are looked into again, and what they have above the bound, again a hundred or
 // two values, is ranked.
 template <typename T>
 __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, const Groups& groups, TopWork& work) {
@@ -203,11 +204,19 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
   const float mine = __shfl_sync(kAll, sortedLanes(top), (of_each - 1) & 31);
   if (lane == 0) work.bound[tid >> 5] = tid >> 5 < warps ? mine : INFINITY;
   __syncthreads();
-  float bound = work.bound[0];
+  unsigned above = 0;
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) bound = fminf(bound, work.bound[w]);
-  if (of_each > 32) bound = -FLT_MAX;
-  bound = fmaxf(bound, -FLT_MAX);  // minus infinity is left to the other way
+  for (int w = 0; w < kWarps; ++w) {
+    const unsigned votes = __ballot_sync(kAll, top >= work.bound[w]);
+    if (lane == w) above = __popc(votes);
+  }
+  if (lane < kWarps) atomicAdd(&work.above[lane], above);
+  __syncthreads();
+  float bound = -FLT_MAX;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+    if ((int)work.above[w] >= k) bound = fmaxf(bound, work.bound[w]);
+  // (minus infinity is left to the other way)
   // A thread's groups side by side in the queue, those of a warp after one addition to its length.
   unsigned pass = 0;
 #pragma unroll
@@ -280,7 +289,6 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
     if (want > 0) selectExactly(sl, want, work);
     n = want;
   }
-  if (tid == 0) work.listed = work.queued = 0;
   for (int i = want + tid; i < k; i += kThreads) work.best[i] = 0;
   rankList(work, n, want);
 }
@@ -375,6 +383,7 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
     TopHook hook;
     hook.groups = &top->groups;
     if (threadIdx.x == 0) top->work.listed = top->work.queued = 0;
+    if (threadIdx.x < kWarps) top->work.above[threadIdx.x] = 0;
     acc = scan<T, kEntropy, kThreads>(sl, c, hook);
     hook.end();
   } else {
