@@ -7,6 +7,10 @@
 // L = sum q_k (log q_k - log p_k) + q_r (log q_r - log p_r); with Q = q_r + sum q_k
 //   dx_v = 1/T (Q p_v - q_v) for a listed token, 1/T (p_v / p_r) (Q p_r - q_r) for any other.
 // p_r is summed from the tokens that are not listed: 1 - sum p_k would lose it where the teacher's tokens are likely.
+//
+// Forward one read of the logits, backward one read and one write; the listed tokens' own logits are read apart, and their
+// gradients written over those of the sweep.  8192 x 51200 bf16, 64 tokens: forward 140 to 147 us, backward 254 (6.6 TB/s; both together
+// 391 us at the copy rate); 2 x 1024 x 51200 with the rest 48 and 61 (91).
 #include "softmax_row.cuh"
 
 namespace fairring {
@@ -72,6 +76,7 @@ template <typename T, int kWidth = kThreads> struct Marks {
   }
 };
 template <int kWidth> struct RestHook {
+  static constexpr int kUnroll = 1;
   const unsigned* bits;
   // Those of what this thread has of batch b.
   template <typename T> __device__ __forceinline__ unsigned listed(int b) const {
@@ -560,7 +565,9 @@ distillation_mean_kernel(const float* __restrict__ loss, const float4* __restric
   }
 }
 
-// A block does one batch of vectors of one row and then, over what it has written, the listed tokens among them.
+// A block does one batch of vectors of one row and then, over what it has written, the listed tokens among them.  What they need is
+// made in the forward, each token once: looking for tokens that are named twice here cost 254 -> 314 us.  The two forms of the exponent as
+// two loops save an instruction a pair and cost the sixth block (42 registers): 256 -> 273 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, const float4* __restrict__ stats,

@@ -2,9 +2,17 @@
 // A = sum of exp((x - m) / T) * log2(exp((x - m) / T)).  Shared by the kernels that ask a language-model head's
 // logits for probabilities.
 //
-// A row is the elements up to its first 16-byte boundary, 16-byte vectors, and what is left behind them.  A
-// block takes a row or, where there are few rows, the blocks of a cluster take a slice of it each and the first
-// one merges what they found, in the order of the slices.
+// A row is the elements up to its first 16-byte boundary, 16-byte vectors, and what is left behind them.  Few rows are taken by a
+// block each or, fewer still, by the blocks of a cluster, a slice each, of which the first merges what they found, in the
+// order of the slices; many by blocks that stay and take row after row; many short ones by a warp each.  Which it is depends on
+// the sizes alone, and so does the order of every sum.
+//
+// What bounds it: the bytes, and next to them the exponentials (16 a clock and multiprocessor: 9 TB/s of bf16 logits) and the
+// instructions around them (about 34 for a vector of 8: unpacking 8, exponents 4, exponentials 8, sums 4, the maximum 5).  8192 rows of
+// 51200 bf16 logits: 134 us, 6.3 TB/s, with the special function unit 60 % and the issue slots 68 % busy; fp32 logits need half the
+// instructions a byte: 2 x 1023 rows of 50265 in 65 us, 6.3 TB/s.  So the instructions are kept few: no comparison of the maximum a value
+// but one a batch, in the logits' own type; two fp32 operations in one instruction (157 us with one, on the form before this); no
+// test for what masked rows need.  A polynomial in place of some exponentials costs more issue slots than it frees (157 -> 178).
 //
 // exp() is 2^((x - m) * c) with c = log2(e) / T, as one fused multiply-add of x, c and the rounded m * c; what that
 // rounding changes all exponentials by is put right at the row's end.  The exponential's own error is 2^-22 of a
@@ -269,7 +277,9 @@ struct Exponent {
 };
 
 // What a kernel does with a batch, that from vector i on, before it is summed; returns its largest value.
+// kUnroll: the batches that a turn of the loop takes.
 struct NoHook {
+  static constexpr int kUnroll = 1;
   template <typename P> __device__ __forceinline__ void begin(const P&) {}
   __device__ __forceinline__ void end() {}
   __device__ __forceinline__ void arrived(uint4*, int) {}
@@ -300,6 +310,7 @@ __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
   };
   ThreadSums acc(c);
   if (whole > 0 || left > 0) fetch(0);
+#pragma unroll Hook::kUnroll
   for (int b = 0; b < whole; ++b) {
 #pragma unroll
     for (int u = 0; u < U; ++u) now[u] = raw[u];
@@ -444,17 +455,17 @@ cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, in
 
 // ---- many rows -----------------------------------------------------------------
 // With a block per row the memory idles while a block starts and while it finishes its row, three to four
-// microseconds of the ten that the row itself takes.  So where there are many rows the blocks stay and take row after row
-// in three roles:
+// microseconds of the ten that the row itself takes.  So where there are many rows the blocks stay, three a multiprocessor, and take
+// row after row (8192 x 51200 bf16: 157 -> 134 us; with the rows dealt out in advance 142) in three roles:
 //  - one warp fetches rows: it asks the hardware for a block that has not started yet and takes over that block's rows,
 //    so that blocks which get more of the memory's bandwidth do more of them; it prepares what needs no look at the logits;
 //  - eight warps sweep: every thread copies its own vectors to shared memory, kDepth - 1 batches ahead and
 //    across the ends of rows, and waits for its own copies alone;
 //  - one warp finishes rows while the next ones are swept.
-constexpr int kManyRows = 4;  // for each multiprocessor
-constexpr int kDepth = 3;
+constexpr int kManyRows = 4;  // for each multiprocessor: 700 rows of 32003 fp32 logits 25.5 us by a block each, 21.5 here; 515 even, 300 the other way
+constexpr int kDepth = 3;     // two batches of 16 KB on their way for each of the three blocks; one more gained nothing
 constexpr int kRowThreads = kThreads + 64;  // sweep, then the warp that fetches, then the one that finishes
-constexpr int kSlots = 3;                   // rows between being fetched and being finished
+constexpr int kSlots = 3;                   // rows between being fetched and being finished; 4 to 6: 134 -> 136 us, with the rest 155 -> 171
 constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait is given up
 
 __device__ __forceinline__ uint32_t sharedAddress(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -736,7 +747,8 @@ inline bool manyRows(int64_t rows, int sm_count) { return rows >= kManyRows * (i
 
 // ---- many short rows -------------------------------------------------------------
 // Up to 16 KB a row is one warp's, which sweeps and finishes it: no thread waits for another warp, and a multiprocessor has 32 rows on
-// the way.
+// the way.  8192 x 1000 bf16 52 -> 6.2 us, the divergence 67 -> 11; at 8192 x 8000 33 us, as much a byte as 8192 x 12000 by the
+// blocks that stay.
 constexpr int kShortBytes = 16384;
 inline bool shortRows(const LogitRows& x, int elem_size, int sm_count) {
   return (int64_t)x.vocab * elem_size <= kShortBytes && manyRows(x.rows, sm_count);
