@@ -356,7 +356,7 @@ distillation_slices_kernel(const T* __restrict__ logits, LogitRows x, Given give
 template <typename T> struct ShortRow {
   Teacher teacher;
   static constexpr int kWords = Marks<T, 32>::words(kShortBytes / 16);
-  unsigned bits[kWords];  // a power of two, and as many bits as a short row has tokens
+  unsigned bits[kWords];
 };
 template <typename T, bool kRest>
 __global__ void __launch_bounds__(kThreads, 4)
@@ -375,14 +375,16 @@ distillation_short_kernel(const T* __restrict__ logits, LogitRows x, Given given
   const T* row = rowOf(x, logits, r);
   const Slice<T> sl(row, x.vocab, 0, 1);
   loadTeacher<T, kRest>(te, given, r, row, x.vocab, (float)inv_t);
-  for (int i = lane; i < ShortRow<T>::kWords; i += 32) mine.bits[i] = 0;
+  constexpr int names = 128;  // words, a power of two
+  static_assert(names <= ShortRow<T>::kWords);
+  for (int i = lane; i < (kRest ? Marks<T, 32>::words(sl.v1) : names); i += 32) mine.bits[i] = 0;
   __syncwarp();
   unsigned left_out = 0;
   bool twice = false;
   if (kRest)
     left_out = markListed<32>(te, k, sl, mine.bits, twice);
   else if (pairs != nullptr)
-    twice = namedTwice(te, k, mine.bits, ShortRow<T>::kWords);
+    twice = namedTwice(te, k, mine.bits, names);
   if (kRest || pairs != nullptr) mergeTeacher(te, k, twice, pairs != nullptr ? pairs + r * k : nullptr);
   Sums acc;
   if constexpr (kRest) {

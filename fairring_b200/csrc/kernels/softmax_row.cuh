@@ -746,12 +746,14 @@ cudaError_t launchRows(void (*kernel)(Params...), int64_t rows, int rows_a_block
 inline bool manyRows(int64_t rows, int sm_count) { return rows >= kManyRows * (int64_t)sm_count; }
 
 // ---- many short rows -------------------------------------------------------------
-// Up to 16 KB a row is one warp's, which sweeps and finishes it: no thread waits for another warp, and a multiprocessor has 32 rows on
-// the way.  8192 x 1000 bf16 52 -> 6.2 us, the divergence 67 -> 11; at 8192 x 8000 33 us, as much a byte as 8192 x 12000 by the
-// blocks that stay.
-constexpr int kShortBytes = 16384;
+// A short row is one warp's, which sweeps and finishes it: no thread waits for another warp, and a multiprocessor has 32 rows on the
+// way.  Up to 16 KB wherever rows are many: 8192 x 1000 bf16 52 -> 6.2 us, the divergence 67 -> 11.  Up to 32 KB with eight rows
+// a multiprocessor, since with fewer the longest rows take longest: 8192 x 12000 53 -> 45 and 70 -> 51, 8192 x 16000 59 -> 58 and
+// 74 -> 63, 1500 x 12000 14.9 -> 13.8 and 19.3 -> 16.2, but 600 x 16000 10.9 -> 14.0 and 14.2 -> 16.3.
+constexpr int kShortBytes = 32768, kVeryShortBytes = 16384;
 inline bool shortRows(const LogitRows& x, int elem_size, int sm_count) {
-  return (int64_t)x.vocab * elem_size <= kShortBytes && manyRows(x.rows, sm_count);
+  const int64_t bytes = (int64_t)x.vocab * elem_size;
+  return bytes <= kShortBytes && x.rows >= (bytes <= kVeryShortBytes ? 1 : 2) * kManyRows * (int64_t)sm_count;
 }
 template <typename... Params, typename... Args>
 cudaError_t launchShort(void (*kernel)(Params...), int64_t rows, size_t shared, cudaStream_t stream, Args... args) {
