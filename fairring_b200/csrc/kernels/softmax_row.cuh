@@ -8,11 +8,12 @@
 // the sizes alone, and so does the order of every sum.
 //
 // What bounds it: the bytes, and next to them the exponentials (16 a clock and multiprocessor: 9 TB/s of bf16 logits) and the
-// instructions around them (about 34 for a vector of 8: unpacking 8, exponents 4, exponentials 8, sums 4, the maximum 5).  8192 rows of
-// 51200 bf16 logits: 134 us, 6.3 TB/s, with the special function unit 60 % and the issue slots 68 % busy; fp32 logits need half the
-// instructions a byte: 2 x 1023 rows of 50265 in 65 us, 6.3 TB/s.  So the instructions are kept few: no comparison of the maximum a value
-// but one a batch, in the logits' own type; two fp32 operations in one instruction (157 us with one, on the form before this); no
-// test for what masked rows need.  A polynomial in place of some exponentials costs more issue slots than it frees (157 -> 178).
+// instructions around them.  8192 rows of 51200 bf16 logits: 134 us, 6.3 TB/s; 61 instructions of a warp for 32 vectors of 8, of them 9
+// for the special function unit, 21 for the multiply-add pipe, 19 integer and comparisons, 4 loads and stores; 60 % of the issue
+// slots.  fp32 logits need half of that a byte: 2 x 1023 rows of 50265 in 65 us, 6.3 TB/s.  So the instructions are kept few: no
+// comparison of the maximum a value but one a batch, in the logits' own type; two fp32 operations in one instruction (157 us at the
+// time, 164 without); no test for what masked rows need.  A polynomial in place of some exponentials costs more issue slots than
+// it frees (157 -> 178).
 //
 // exp() is 2^((x - m) * c) with c = log2(e) / T, as one fused multiply-add of x, c and the rounded m * c; what that
 // rounding changes all exponentials by is put right at the row's end.  The exponential's own error is 2^-22 of a

@@ -6,7 +6,7 @@
 //
 // Forward one read of the logits, backward one read and one write.  4 x 1024 x 51200 bf16 with the entropy, a quarter of the rows
 // not counting: forward 68 us, backward 125 (5.9 TB/s; both together 163 us at the copy rate); 8192 x 51200 with
-// the 64 largest entries 194 us (131 at the copy rate).
+// the 64 largest entries 188 us (131 at the copy rate).
 #include <cfloat>
 #include <cmath>
 
@@ -37,9 +37,9 @@ __device__ __forceinline__ uint64_t entryOf(float v, int col) { return (uint64_t
 
 // Where the entries that are asked for are found: the sweep leaves the largest value of every thread's groups of columns, from these
 // comes a bound, and only the groups that reach it are read again, from L2.  It is the block's own work, with the row's
-// candidates in shared memory, five blocks a multiprocessor; 42.7 million instructions for 2048 rows of 51200, about 7000 of the
-// 20800 a row the sweep's.  Warps of blocks that stay doing this behind the sweep were slower (274 us and more against 220 then), and so
-// was keeping vectors above a bound while sweeping (245 against 208).
+// candidates in shared memory, five blocks a multiprocessor.  2048 rows of 51200 bf16 logits: 41.8 million instructions of a warp with 64
+// entries, 35.8 with one, 25.0 for the log probabilities alone.  Warps of blocks that stay doing this behind the sweep were
+// slower (274 us and more against 220 then), and so was keeping vectors above a bound while sweeping (245 against 208).
 struct Groups {
   float top[kGroups][kThreads];
 };
