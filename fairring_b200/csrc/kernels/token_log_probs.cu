@@ -21,6 +21,7 @@ constexpr int kMostTop = kMostTopTokens;
 constexpr int kGroups = 8;    // largest values that a sweeping thread leaves of a row
 constexpr int kQueue = 512;   // groups of columns that are looked into
 constexpr int kList = 1024;   // candidates that are ranked
+constexpr int kShortList = 256;  // of a row that one warp has
 static_assert(kList >= kMostSlices * kMostTop, "the slices' results are candidates");
 
 // Order of logits as unsigned integers: NaN above everything, both zeros alike.
@@ -43,15 +44,24 @@ __device__ __forceinline__ uint64_t entryOf(float v, int col) { return (uint64_t
 struct Groups {
   float top[kGroups][kThreads];
 };
-struct TopWork {
-  alignas(16) uint64_t list[kList];
+// Of kWidth threads, a block's or a warp's.
+template <int kEntries> struct Candidates {
+  alignas(16) uint64_t list[kEntries];
   uint64_t best[kMostTop];  // the result, in falling order
   unsigned hist[256];
+  unsigned listed, digit, left;
+};
+struct TopWork : Candidates<kList> {
   int queue[kQueue];
   float bound[kWarps];
-  unsigned above[kWarps];
-  unsigned queued, listed, digit, left;
+  unsigned above[kWarps], queued;
 };
+template <int kWidth> __device__ __forceinline__ void syncWidth() {
+  if constexpr (kWidth == 32)
+    __syncwarp();
+  else
+    __syncthreads();
+}
 
 // Falling order of 32 values, one per lane.
 __device__ __forceinline__ float sortedLanes(float v) {
@@ -99,14 +109,15 @@ struct TopHook {
 };
 
 // The `want` largest of the first n entries of the list, in falling order, to `best`.
-__device__ __forceinline__ void rankList(TopWork& work, int n, int want) {
+template <int kWidth, int kEntries> __device__ __forceinline__ void rankList(Candidates<kEntries>& work, int n, int want) {
+  const int tid = threadIdx.x % kWidth;
   uint64_t* list = work.list;
-  if (n <= 2 * kThreads) {  // every entry counts those above it, two threads an entry where there are threads enough
-    if ((int)threadIdx.x == 0 && (n & 1)) list[n] = 0;
-    if (n & 1) __syncthreads();
-    const bool split = 2 * n <= kThreads;
-    const int pairs = (n + 1) / 2, from = split && ((int)threadIdx.x & 1) ? pairs / 2 : 0, to = split && !((int)threadIdx.x & 1) ? pairs / 2 : pairs;
-    for (int i = split ? (int)threadIdx.x / 2 : (int)threadIdx.x; i < (split ? kThreads / 2 : (n + 31) / 32 * 32); i += kThreads) {
+  if (n <= (kWidth == 32 ? 64 : 2 * kWidth)) {  // every entry counts those above it, two threads an entry where there are threads enough
+    if (tid == 0 && (n & 1)) list[n] = 0;
+    if (n & 1) syncWidth<kWidth>();
+    const bool split = 2 * n <= kWidth;
+    const int pairs = (n + 1) / 2, from = split && (tid & 1) ? pairs / 2 : 0, to = split && !(tid & 1) ? pairs / 2 : pairs;
+    for (int i = split ? tid / 2 : tid; i < (split ? kWidth / 2 : (n + 31) / 32 * 32); i += kWidth) {
       const uint64_t mine = i < n ? list[i] : 0;
       int above = 0;
 #pragma unroll 4
@@ -118,40 +129,41 @@ __device__ __forceinline__ void rankList(TopWork& work, int n, int want) {
       if (split) above += __shfl_xor_sync(kAll, above, 1);
       if (i < n && above < want) work.best[above] = mine;
     }
-    __syncthreads();
+    syncWidth<kWidth>();
     return;
   }
   int size = 2;
   while (size < n) size *= 2;
-  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) list[i] = 0;
-  __syncthreads();
+  for (int i = n + tid; i < size; i += kWidth) list[i] = 0;
+  syncWidth<kWidth>();
   for (int block = 2; block <= size; block *= 2)
     for (int step = block / 2; step > 0; step /= 2) {
-      for (int i = (int)threadIdx.x; i < size / 2; i += kThreads) {
+      for (int i = tid; i < size / 2; i += kWidth) {
         const int a = 2 * i - (i & (step - 1)), b = a + step;
         const uint64_t x = list[a], y = list[b];
         if ((x < y) == ((a & block) == 0)) list[a] = y, list[b] = x;
       }
-      __syncthreads();
+      syncWidth<kWidth>();
     }
-  for (int i = (int)threadIdx.x; i < want; i += kThreads) work.best[i] = list[i];
-  __syncthreads();
+  for (int i = tid; i < want; i += kWidth) work.best[i] = list[i];
+  syncWidth<kWidth>();
 }
 
 // The `want` largest of the slice's entries, to the list in any order, by a radix select that reads the slice six
 // times and more: for rows where the bound lets too much pass (ties, rising logits) and those with NaN.
-template <typename T> __device__ __noinline__ void selectExactly(const Slice<T>& sl, int want, TopWork& work) {
-  const int tid = threadIdx.x, lane = threadIdx.x & 31;
+template <int kWidth, typename T, int kEntries>
+__device__ __noinline__ void selectExactly(const Slice<T>& sl, int want, Candidates<kEntries>& work) {
+  const int tid = threadIdx.x % kWidth, lane = threadIdx.x & 31;
   uint32_t prefix = 0;
   unsigned left = want;
   for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kThreads) work.hist[i] = 0;
-    __syncthreads();
-    for (int col = sl.c0 + tid; col < sl.c1; col += kThreads) {
+    for (int i = tid; i < 256; i += kWidth) work.hist[i] = 0;
+    syncWidth<kWidth>();
+    for (int col = sl.c0 + tid; col < sl.c1; col += kWidth) {
       const uint32_t key = keyOf(toFloat(sl.row[col]));
       if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&work.hist[key >> shift & 255u], 1u);
     }
-    __syncthreads();
+    syncWidth<kWidth>();
     if (tid == 0) {
       int digit = 255;
       unsigned more = left;
@@ -159,37 +171,37 @@ template <typename T> __device__ __noinline__ void selectExactly(const Slice<T>&
       work.digit = digit;
       work.left = more;
     }
-    __syncthreads();
+    syncWidth<kWidth>();
     prefix = prefix << 8 | work.digit;
     left = work.left;
-    __syncthreads();
+    syncWidth<kWidth>();
   }
   // `prefix` is the key of the last one; `left` of those that equal it are taken, the first ones.
   if (tid == 0) work.listed = 0;
-  __syncthreads();
-  for (int col = sl.c0 + tid; col < sl.c1; col += kThreads) {
+  syncWidth<kWidth>();
+  for (int col = sl.c0 + tid; col < sl.c1; col += kWidth) {
     const float v = toFloat(sl.row[col]);
     if (keyOf(v) > prefix) work.list[atomicAdd(&work.listed, 1u)] = entryOf(v, col);
   }
   const unsigned larger = want - left;
   unsigned taken = 0;
-  for (int base = sl.c0; base < sl.c1 && taken < left; base += kThreads) {
+  for (int base = sl.c0; base < sl.c1 && taken < left; base += kWidth) {
     const int col = base + tid;
     const float v = col < sl.c1 ? toFloat(sl.row[col]) : 0.f;
     const bool equal = col < sl.c1 && keyOf(v) == prefix;
     const unsigned votes = __ballot_sync(kAll, equal);
-    __syncthreads();
+    syncWidth<kWidth>();
     if (lane == 0) work.hist[tid >> 5] = __popc(votes);
-    __syncthreads();
+    syncWidth<kWidth>();
     unsigned before = taken + __popc(votes & ((1u << lane) - 1u)), all = 0;
-    for (int w = 0; w < kThreads / 32; ++w) {
+    for (int w = 0; w < kWidth / 32; ++w) {
       if (w < tid >> 5) before += work.hist[w];
       all += work.hist[w];
     }
     if (equal && before < left) work.list[larger + before] = entryOf(v, col);
     taken += all;
   }
-  __syncthreads();
+  syncWidth<kWidth>();
 }
 
 // The slice's largest entries, at most k, in falling order, to `best`, zeros behind them up to k.  The sweep is over for all of the
@@ -296,11 +308,11 @@ __device__ __forceinline__ void sliceTop(const Slice<T>& sl, int k, bool nan, co
   int n = work.listed;
   __syncthreads();
   if (nan || !fits || n > kList || n < want) {
-    if (want > 0) selectExactly(sl, want, work);
+    if (want > 0) selectExactly<kThreads>(sl, want, work);
     n = want;
   }
   for (int i = want + tid; i < k; i += kThreads) work.best[i] = 0;
-  rankList(work, n, want);
+  rankList<kThreads>(work, n, want);
 }
 
 // The k largest of the row from the slices' results, in block 0.  clusterSums() has waited for those.
@@ -314,7 +326,124 @@ __device__ __forceinline__ void clusterTop(int k, TopWork& work) {
     work.list[i] = cluster.map_shared_rank(&work, r)->best[i - r * k];
   }
   __syncthreads();
-  rankList(work, slices * k, k);
+  rankList<kThreads>(work, slices * k, k);
+}
+
+// The same for a row that one warp has.  Its groups are `span` of a lane's vectors, a power of two.
+struct WarpTopHook {
+  static constexpr int kUnroll = 1;
+  float (*groups)[32];
+  int span = 1, at = 0;  // `at`: the vector that comes next
+  float top = -INFINITY;
+  template <typename T> static __device__ __forceinline__ int vectors(const Slice<T>& sl) { return (sl.v1 - sl.v0 + 31) / 32; }
+  template <typename T> static __device__ __forceinline__ int spanOf(const Slice<T>& sl) {
+    int span = 1;
+    while (span * kGroups < vectors(sl)) span *= 2;
+    return span;
+  }
+  template <typename T> __device__ __forceinline__ float batch(const uint4 (&now)[kBatch], bool first, int, const Slice<T>& sl) {
+    const int lane = threadIdx.x & 31;
+    if (first) span = spanOf(sl);
+    float m[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) m[u] = Vec<T>::max(now[u]);
+    const float low = fmaxf(m[0], m[1]), high = fmaxf(m[2], m[3]), largest = fmaxf(low, high);
+    if (span >= kBatch) {
+      top = fmaxf(top, largest);
+      if ((at + kBatch) % span == 0) groups[at / span][lane] = top, top = -INFINITY;
+    } else if (span == 2) {
+      groups[at / 2][lane] = low;
+      groups[at / 2 + 1][lane] = high;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) groups[at + u][lane] = m[u];
+    }
+    at += kBatch;
+    return largest;
+  }
+  __device__ __forceinline__ void end() {
+    if (at % span != 0) groups[at / span][threadIdx.x & 31] = top;
+  }
+};
+static_assert(kBatch == 4 && kGroups == 8, "a batch is one group, two, or a part of one");
+
+// Its k largest entries.  The bound is the k-th of the lanes' largest, or for more entries the best of the groups' as the warps' above.
+constexpr int kFew = 24;  // 20 entries of 8192 x 1000: 18 us so, 23 by the groups
+template <typename T>
+__device__ __forceinline__ void warpTop(const Slice<T>& sl, int k, bool nan, const float (*groups)[32], Candidates<kShortList>& work) {
+  constexpr int E = Vec<T>::kElems;
+  const int lane = threadIdx.x & 31, vectors = WarpTopHook::vectors(sl), span = WarpTopHook::spanOf(sl);
+  const int number = (vectors + span - 1) / span, at_work = (sl.v1 - sl.v0) / 32;  // vectors that every lane has
+  float value[kGroups], top = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    value[g] = g < number ? groups[g][lane] : -INFINITY;
+    top = fmaxf(top, value[g]);
+  }
+  float bound = -FLT_MAX;
+  if (k <= kFew) {
+    if (at_work > 0) bound = fmaxf(bound, __shfl_sync(kAll, sortedLanes(top), k - 1));
+  } else {
+    const int full = (at_work + span - 1) / span, of_each = full > 0 ? (k + full - 1) / full : 33;
+#pragma unroll 1
+    for (int g = 0; g < full && of_each <= 32; ++g) {
+      const float mine = __shfl_sync(kAll, sortedLanes(groups[g][lane]), of_each - 1);
+      int above = 0;
+#pragma unroll
+      for (int h = 0; h < kGroups; ++h) above += __popc(__ballot_sync(kAll, value[h] >= mine));
+      if (above >= k) bound = fmaxf(bound, mine);
+    }
+  }
+  // Every lane looks again into its own groups that reach the bound.
+  const uint4* all = reinterpret_cast<const uint4*>(sl.row + sl.head);
+  int listed = 0;
+  auto list = [&](unsigned mask, auto colOf) {
+    int pos = __popc(mask);
+    if (!__any_sync(kAll, mask != 0)) return;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int below = __shfl_up_sync(kAll, pos, o);
+      if (lane >= o) pos += below;
+    }
+    const int found = __shfl_sync(kAll, pos, 31);
+    for (pos += listed - __popc(mask); mask != 0; mask &= mask - 1, ++pos) {
+      const int col = colOf(__ffs(mask) - 1);
+      if (pos < kShortList) work.list[pos] = entryOf(toFloat(sl.row[col]), col);
+    }
+    listed += found;
+    __syncwarp();
+  };
+#pragma unroll 1
+  for (int b = 0; b < vectors; b += kBatch) {
+    bool pass[kBatch], any = false;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      pass[u] = b + u < vectors && sl.v0 + (b + u) * 32 + lane < sl.v1 && groups[(b + u) / span][lane] >= bound;
+      any |= pass[u];
+    }
+    if (!__any_sync(kAll, any)) continue;
+    uint4 raw[kBatch];
+    constexpr uint32_t w = Vec<T>::kMinusInf;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) raw[u] = pass[u] ? all[sl.v0 + (b + u) * 32 + lane] : make_uint4(w, w, w, w);
+    unsigned mask = 0;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float2 v[E / 2];
+      Vec<T>::get(raw[u], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) mask |= (e & 1 ? v[e / 2].y : v[e / 2].x) >= bound ? 1u << (u * E + e) : 0u;
+    }
+    list(mask, [&](int bit) { return sl.head + (sl.v0 + (b + bit / E) * 32 + lane) * E + bit % E; });
+  }
+  const int loose = lane < 2 * E ? sl.looseCol(lane) : -1;
+  list(loose >= 0 && toFloat(sl.row[loose]) >= bound ? 1u : 0u, [&](int) { return loose; });
+  int n = listed;
+  if (nan || n > kShortList || n < k) {
+    selectExactly<32>(sl, k, work);
+    n = k;
+  }
+  rankList<32>(work, n, k);
 }
 
 // What one row leaves; any pointer but `tokens` may be null.  Kept for the backward: m and S as its exponents need it, which is
@@ -352,10 +481,10 @@ struct Outputs {
     if (kEntropy) entropy[r] = low - acc.a / acc.s * kLn2;
     if (stats != nullptr) stats[r] = make_float2(acc.m, known ? acc.s * exp2Of(Exponent::excess(acc.m, c)) : nan);
   }
-  // By a block.
-  __device__ __forceinline__ void largest(int64_t r, const Sums& acc, const uint64_t* best, float inv_t) const {
+  // By a block or a warp.
+  template <int kWidth> __device__ __forceinline__ void largest(int64_t r, const Sums& acc, const uint64_t* best, float inv_t) const {
     const float low = logf(acc.s);
-    for (int i = (int)threadIdx.x; i < k; i += kThreads) {
+    for (int i = (int)threadIdx.x % kWidth; i < k; i += kWidth) {
       const uint64_t entry = best[i];
       top_log_probs[r * k + i] = fmaf(valueOf((uint32_t)(entry >> 32)) - acc.m, inv_t, -low);
       top_tokens[r * k + i] = (int)~(uint32_t)entry;
@@ -414,13 +543,18 @@ token_log_probs_slices_kernel(const T* __restrict__ logits, LogitRows x, Outputs
   }
   if (!acc.template settle<kEntropy>(c)) acc = blockAgain<T, kEntropy>(sl.row, x.vocab, c, scratch, LeaveNone());
   if (threadIdx.x == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
-  if constexpr (kTop) out.largest(r, acc, top->work.best, inv_t);
+  if constexpr (kTop) out.template largest<kThreads>(r, acc, top->work.best, inv_t);
 }
 
 // Many short rows: one per warp.
-template <typename T, bool kEntropy>
+struct ShortTop {
+  Candidates<kShortList> work;
+  float groups[kGroups][32];
+};
+template <typename T, bool kEntropy, bool kTop>
 __global__ void __launch_bounds__(kThreads, 4)
 token_log_probs_short_kernel(const T* __restrict__ logits, LogitRows x, Outputs out, float c, float inv_t) {
+  extern __shared__ __align__(16) unsigned char dynamic[];
   const int lane = threadIdx.x & 31;
   const int64_t r = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (r >= x.rows) return;
@@ -432,13 +566,33 @@ token_log_probs_short_kernel(const T* __restrict__ logits, LogitRows x, Outputs 
   const Slice<T> sl(rowOf(x, logits, r), x.vocab, 0, 1);
   const bool known = t < x.vocab;
   const float logit = known ? toFloat(sl.row[t]) : 0.f;
-  NoHook none;
-  Sums acc = scan<T, kEntropy, 32>(sl, c, none);
+  ShortTop* top = reinterpret_cast<ShortTop*>(dynamic) + (threadIdx.x >> 5);
+  Sums acc;
+  if constexpr (kTop) {
+    WarpTopHook hook;
+    hook.groups = top->groups;
+    acc = scan<T, kEntropy, 32>(sl, c, hook);
+    hook.end();
+  } else {
+    NoHook none;
+    acc = scan<T, kEntropy, 32>(sl, c, none);
+  }
   const int col = lane < 2 * Vec<T>::kElems ? sl.looseCol(lane) : -1;
   if (col >= 0) acc.add<kEntropy>(toFloat(sl.row[col]), c);
   acc = warpSums<kEntropy>(acc, c);
+  if constexpr (kTop) warpTop(sl, out.k, acc.s != acc.s, top->groups, top->work);
   if (!acc.template settle<kEntropy>(c)) acc = warpAgain<T, kEntropy>(sl.row, x.vocab, c, LeaveNone());
   if (lane == 0) out.values<kEntropy>(r, acc, known, logit, c, inv_t);
+  if constexpr (kTop) out.template largest<32>(r, acc, top->work.best, inv_t);
+}
+
+// One warp is slow with long rows and many entries, but a multiprocessor has 32 of them: up to 1 KB for each row that a
+// multiprocessor gets, and 24 KB.  bf16, 20 entries: 8192 x 1000 85 -> 18 us, 8192 x 8000 94 -> 62, 2500 x 4000 29 -> 18,
+// 600 x 1000 10 -> 6; but 8192 x 16000 110 -> 118, 1200 x 8000 17 -> 26.  More entries than 64 overflow a warp's list where
+// rows are not short (8192 x 8000, 128 entries: 165 -> 341).
+inline bool shortTop(const LogitRows& x, int k, int elem_size, int sm_count) {
+  const int64_t bytes = (int64_t)x.vocab * elem_size;
+  return k <= 64 && manyRows(x.rows, sm_count) && bytes <= 24 * 1024 && bytes <= 1024 * (x.rows / sm_count);
 }
 
 // Many rows: the blocks stay.
@@ -551,7 +705,9 @@ template <typename T, bool kEntropy>
 cudaError_t forwardOf(const T* logits, const LogitRows& x, const Outputs& out, double temperature, int sm_count, cudaStream_t stream) {
   const float inv_t = (float)(1.0 / temperature), c = (float)(1.4426950408889634 / temperature);
   if (out.k == 0 && shortRows(x, sizeof(T), sm_count))
-    return launchShort(token_log_probs_short_kernel<T, kEntropy>, x.rows, 0, stream, logits, x, out, c, inv_t);
+    return launchShort(token_log_probs_short_kernel<T, kEntropy, false>, x.rows, 0, stream, logits, x, out, c, inv_t);
+  if (out.k > 0 && shortTop(x, out.k, sizeof(T), sm_count))
+    return launchShort(token_log_probs_short_kernel<T, kEntropy, true>, x.rows, kWarps * sizeof(ShortTop), stream, logits, x, out, c, inv_t);
   if (out.k == 0 && manyRows(x.rows, sm_count)) {
     const int rows_a_block = rowsABlock(x, sizeof(T), sm_count);
     return launchRows(token_log_probs_rows_kernel<T, kEntropy>, x.rows, rows_a_block, sizeof(Rows), stream, logits, x, out, c, inv_t,

@@ -449,3 +449,38 @@ def test_a_vocabulary_past_the_kernels():
     x = torch.zeros(1, device="cuda").expand(1, _C.MOST_VOCAB + 1)
     with pytest.raises(ValueError):
         _C.token_log_probs(x, torch.zeros(1, dtype=torch.long, device="cuda"), 1.0, False, 0)
+
+
+@pytest.mark.parametrize("vocab", [1, 31, 255, 264, 1025, 2051, 4099, 8200])
+@pytest.mark.parametrize("k", [1, 24, 25, 64])
+@pytest.mark.parametrize("kind", ["spread", "equal", "few values", "rising", "few left", "not a number"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_top_of_many_short_rows(vocab, k, kind, dtype):
+    """One warp a row: vectors that some lanes lack, groups of 1, 2, 4 and 8 vectors, lists that overflow."""
+    from fairring_b200.ops import token_log_probs
+
+    rows, k = 5000, min(k, vocab)
+    x = _logits(rows, vocab, dtype)
+    if kind == "equal":
+        x.zero_()
+    elif kind == "few values":
+        x = x.sign()
+    elif kind == "rising":
+        x = torch.arange(vocab, device="cuda").expand(rows, vocab).to(dtype).contiguous()
+    elif kind == "few left":
+        x[:, 3:] = float("-inf")
+    elif kind == "not a number":
+        x[::3, vocab // 3] = float("nan")
+        x[1::3, vocab // 2] = float("inf")
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(3))
+    tokens[::7] = -100
+    got = token_log_probs(x, tokens, temperature=0.8, top_k=k, entropy=True)
+    counts = tokens >= 0
+    order = x.sort(dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(got.top_tokens, torch.where(counts[:, None], order, -1))
+    logp = (x.double() / 0.8).log_softmax(-1)
+    want = torch.where(counts[:, None], logp.gather(1, order), float("-inf"))
+    # as _check() has it for the log probabilities
+    torch.testing.assert_close(got.top_log_probs.double(), want, rtol=4 * 2.0 ** -24, atol=2.0 ** -17.3, equal_nan=True)
+    of = torch.where(counts, logp.gather(1, tokens.clamp_min(0)[:, None])[:, 0], 0.0)
+    torch.testing.assert_close(got.log_probs.double(), of, rtol=4 * 2.0 ** -24, atol=2.0 ** -17.3, equal_nan=True)
