@@ -277,6 +277,31 @@ struct Exponent {
   }
 };
 
+// A barrier of a warp or a block.
+template <int kWidth> __device__ __forceinline__ void syncWidth() {
+  if constexpr (kWidth == 32)
+    __syncwarp();
+  else
+    __syncthreads();
+}
+
+// Backward: rows in pieces of kBatch vectors for each of a warp's threads, numbered through all rows.  The numbers are of 32
+// bits, since a division of 64 takes as long as a vector: 2^31 rows, and 2 KB of logits to each piece past a row's first.
+struct Pieces {
+  unsigned total, a_row;
+  // False if there are too many.
+  template <typename T> bool cut(const LogitRows& x) {
+    constexpr int per_piece = 32 * kBatch * Vec<T>::kElems;
+    const int64_t each = ((int64_t)x.vocab + per_piece - 1) / per_piece;
+    if (each > (int64_t)(UINT32_MAX - kThreads) / x.rows) return false;
+    a_row = (unsigned)each;
+    total = (unsigned)(x.rows * each);
+    return true;
+  }
+  unsigned blocks() const { return (total + kWarps - 1) / kWarps; }
+  static __device__ __forceinline__ unsigned mine() { return blockIdx.x * kWarps + threadIdx.x / 32; }
+};
+
 // What a kernel does with a batch, that from vector i on, before it is summed; returns its largest value.
 // kUnroll: the batches that a turn of the loop takes.
 struct NoHook {

@@ -5,7 +5,7 @@
 // terms that are not negative.  Backward:  dx_v = 1/T [ g (1[v = t] - p_v) - h p_v (log p_v + H) ].
 //
 // Forward one read of the logits, backward one read and one write.  4 x 1024 x 51200 bf16 with the entropy, a quarter of the rows
-// not counting: forward 68 us, backward 125 (5.9 TB/s; both together 163 us at the copy rate); 8192 x 51200 with
+// not counting: forward 68 us, backward 121 (6.1 TB/s; both together 163 us at the copy rate); 8192 x 51200 with
 // the 64 largest entries 188 us (131 at the copy rate).
 #include <cfloat>
 #include <cmath>
@@ -56,12 +56,6 @@ struct TopWork : Candidates<kList> {
   float bound[kWarps];
   unsigned above[kWarps], queued;
 };
-template <int kWidth> __device__ __forceinline__ void syncWidth() {
-  if constexpr (kWidth == 32)
-    __syncwarp();
-  else
-    __syncthreads();
-}
 
 // Falling order of 32 values, one per lane.
 __device__ __forceinline__ float sortedLanes(float v) {
@@ -633,71 +627,72 @@ token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs o
   });
 }
 
-// A block does one batch of vectors of one row, so that all blocks are alike whatever the vocabulary.  With the entropy six
-// blocks a multiprocessor (40 registers); without it the compiler's 56 registers and four are as fast.
+// A warp does one batch of vectors of one row, so that all are alike whatever the vocabulary; a block a batch of 16 KB left threads
+// idle at the row's end: 4 x 1024 x 51200 125 -> 121 us, 8192 x 8200 bf16 58 -> 44, 8192 x 1000 22 -> 7.  Six blocks a
+// multiprocessor (40 registers); with the 56 that it would take without the entropy 8192 x 20000 fp32 took 210 us and now takes 185.
 template <typename T, bool kEntropy>
-__global__ void __launch_bounds__(kThreads, kEntropy ? 6 : 1)
+__global__ void __launch_bounds__(kThreads, 6)
 token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restrict__ grad,
                            const int64_t* __restrict__ tokens, const float2* __restrict__ stats,
                            const float* __restrict__ entropy, const float* __restrict__ g_log_probs, int64_t g_stride,
-                           const float* __restrict__ g_entropy, int64_t h_stride, float c, float inv_t,
-                           int64_t pieces_total, int pieces) {
-  constexpr int E = Vec<T>::kElems, U = kBatch;
-  for (int64_t w = blockIdx.x; w < pieces_total; w += gridDim.x) {
-    const int64_t r = w / pieces;
-    const int piece = (int)(w - r * pieces);
-    const T* row = rowOf(x, logits, r);
-    T* out = rowOf(x, grad, r);
-    const RowParts<T> parts(row, x.vocab);
-    const int first = piece * U * kThreads + (int)threadIdx.x;
-    const uint4* vecs = reinterpret_cast<const uint4*>(row + parts.head);
-    uint4* vout = reinterpret_cast<uint4*>(out + parts.head);
-    const float2 st = stats[r];
-    const bool counts = !(st.y == -1.f);
-    uint4 raw[U];
+                           const float* __restrict__ g_entropy, int64_t h_stride, float c, float inv_t, Pieces pieces) {
+  constexpr int E = Vec<T>::kElems, U = kBatch, kWidth = 32;
+  const int tid = threadIdx.x % kWidth;
+  const unsigned w = pieces.mine();
+  if (w >= pieces.total) return;
+  const int64_t r = w / pieces.a_row;
+  const int piece = (int)(w % pieces.a_row);
+  const T* row = rowOf(x, logits, r);
+  T* out = rowOf(x, grad, r);
+  const RowParts<T> parts(row, x.vocab);
+  const int first = piece * U * kWidth + tid;
+  const uint4* vecs = reinterpret_cast<const uint4*>(row + parts.head);
+  uint4* vout = reinterpret_cast<uint4*>(out + parts.head);
+  const float2 st = stats[r];
+  const bool counts = !(st.y == -1.f);
+  uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      raw[u] = counts && first + u * kThreads < parts.nvec ? __ldg(vecs + first + u * kThreads) : make_uint4(0, 0, 0, 0);
-    const float g = g_log_probs != nullptr ? g_log_probs[r * g_stride] * inv_t : 0.f;
-    const float h = kEntropy ? g_entropy[r * h_stride] * inv_t : 0.f;
-    const int64_t t64 = tokens != nullptr ? tokens[r] : -1;
-    const int t = t64 < x.vocab ? (int)t64 : -1;
-    // g (1[v = t] - p) - h p (log p + H) with p = e / S and log p = u ln 2 - log S, u the exponent of e
-    const float per_s = 1.f / st.y;
-    const float a = -(kEntropy ? fmaf(h, entropy[r] - logf(st.y), g) : g) * per_s, b = -h * kLn2 * per_s;
-    const Exponent exponent(st.x, c);
-    auto of = [&](float2 v) {
-      const float2 d = exponent(v), e = make_float2(exp2Of(d.x), exp2Of(d.y));
-      if (!kEntropy) return mul2(e, make_float2(a, a));
-      return mul2(e, fma2(make_float2(fmaxf(d.x, kLowExponent), fmaxf(d.y, kLowExponent)), make_float2(b, b), make_float2(a, a)));
-    };
+  for (int u = 0; u < U; ++u)
+    raw[u] = counts && first + u * kWidth < parts.nvec ? __ldg(vecs + first + u * kWidth) : make_uint4(0, 0, 0, 0);
+  const float g = g_log_probs != nullptr ? g_log_probs[r * g_stride] * inv_t : 0.f;
+  const float h = kEntropy ? g_entropy[r * h_stride] * inv_t : 0.f;
+  const int64_t t64 = tokens != nullptr ? tokens[r] : -1;
+  const int t = t64 < x.vocab ? (int)t64 : -1;
+  // g (1[v = t] - p) - h p (log p + H) with p = e / S and log p = u ln 2 - log S, u the exponent of e
+  const float per_s = 1.f / st.y;
+  const float a = -(kEntropy ? fmaf(h, entropy[r] - logf(st.y), g) : g) * per_s, b = -h * kLn2 * per_s;
+  const Exponent exponent(st.x, c);
+  auto of = [&](float2 v) {
+    const float2 d = exponent(v), e = make_float2(exp2Of(d.x), exp2Of(d.y));
+    if (!kEntropy) return mul2(e, make_float2(a, a));
+    return mul2(e, fma2(make_float2(fmaxf(d.x, kLowExponent), fmaxf(d.y, kLowExponent)), make_float2(b, b), make_float2(a, a)));
+  };
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = first + u * kThreads;
-      if (i >= parts.nvec) continue;
-      uint4 result = make_uint4(0, 0, 0, 0);
-      if (counts) {
-        float2 v[E / 2];
-        Vec<T>::get(raw[u], v);
-        const int at = t - (parts.head + i * E);
+  for (int u = 0; u < U; ++u) {
+    const int i = first + u * kWidth;
+    if (i >= parts.nvec) continue;
+    uint4 result = make_uint4(0, 0, 0, 0);
+    if (counts) {
+      float2 v[E / 2];
+      Vec<T>::get(raw[u], v);
+      const int at = t - (parts.head + i * E);
 #pragma unroll
-        for (int k = 0; k < E / 2; ++k) v[k] = of(v[k]);
-        if ((unsigned)at < (unsigned)E) {
+      for (int k = 0; k < E / 2; ++k) v[k] = of(v[k]);
+      if ((unsigned)at < (unsigned)E) {
 #pragma unroll
-          for (int k = 0; k < E / 2; ++k) {
-            if (at == 2 * k) v[k].x += g;
-            if (at == 2 * k + 1) v[k].y += g;
-          }
+        for (int k = 0; k < E / 2; ++k) {
+          if (at == 2 * k) v[k].x += g;
+          if (at == 2 * k + 1) v[k].y += g;
         }
-        result = Vec<T>::set(v);
       }
-      vout[i] = result;
+      result = Vec<T>::set(v);
     }
-    if (piece == 0 && threadIdx.x < 2 * E) {
-      const int i = threadIdx.x, col = i < parts.head ? i : i + parts.nvec * E;
-      if (col < x.vocab)
-        fromFloat(out + col, counts ? of(make_float2(toFloat(row[col]), 0.f)).x + (col == t ? g : 0.f) : 0.f);
-    }
+    vout[i] = result;
+  }
+  if (piece == 0 && tid < 2 * E) {
+    const int i = tid, col = i < parts.head ? i : i + parts.nvec * E;
+    if (col < x.vocab)
+      fromFloat(out + col, counts ? of(make_float2(toFloat(row[col]), 0.f)).x + (col == t ? g : 0.f) : 0.f);
   }
 }
 
@@ -730,15 +725,13 @@ cudaError_t forwardOf(const void* logits, const LogitRows& x, const TokenLogProb
 
 template <typename T>
 cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const TokenLogProbsGrads& a, cudaStream_t stream) {
-  constexpr int per_piece = kThreads * kBatch * Vec<T>::kElems;
-  const int pieces = (int)(((int64_t)x.vocab + per_piece - 1) / per_piece);
-  const int64_t total = x.rows * pieces;
-  const unsigned blocks = (unsigned)(total < (1 << 30) ? total : (1 << 30));
+  Pieces pieces;
+  if (!pieces.template cut<T>(x)) return cudaErrorInvalidValue;
   const float inv_t = (float)(1.0 / a.temperature), c = (float)(1.4426950408889634 / a.temperature);
   auto run = [&](auto kernel) {
-    kernel<<<blocks, kThreads, 0, stream>>>(static_cast<const T*>(logits), x, static_cast<T*>(grad), a.tokens,
+    kernel<<<pieces.blocks(), kThreads, 0, stream>>>(static_cast<const T*>(logits), x, static_cast<T*>(grad), a.tokens,
                                             reinterpret_cast<const float2*>(a.stats), a.entropy, a.g_log_probs, a.g_stride,
-                                            a.g_entropy, a.h_stride, c, inv_t, total, pieces);
+                                            a.g_entropy, a.h_stride, c, inv_t, pieces);
     noteLocalLaunch();
     return cudaGetLastError();
   };
