@@ -17,9 +17,10 @@
 //
 // exp() is 2^((x - m) * c) with c = log2(e) / T, as one fused multiply-add of x, c and the rounded m * c; what that
 // rounding changes all exponentials by is put right at the row's end.  The exponential's own error is 2^-22 of a
-// probability.  That form needs |m * c| < 2^20.  A thread's m starts at -2^20 / c, below which nothing is seen of a row unless
-// all of it is there; such rows (masked with the type's lowest value throughout, or with minus infinity), those above and those with
-// a NaN come out of the sweep with a sum that is no positive number and are looked at again, slowly.
+// probability.  That form needs |m * c| < 2^20.  A thread's m starts at -2^20 / c.  A row whose largest value is above has a sum of 1 or
+// more, but for roundings.  One whose largest value is below (masked with the type's lowest value or with minus infinity throughout,
+// say) has lost its smaller values to zero, and all of them from 126 / c below on: its sum is smaller than 1/2 unless it has lost nothing
+// that fp32 sees, and it is looked at again, slowly, as are rows above that range and those with a NaN.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -222,7 +223,7 @@ struct Sums {
   // Relative to m; false for a row that has to be looked at again.
   template <bool kEntropy> __device__ __forceinline__ bool settle(float c) {
     shift<kEntropy>(-fmaf(m, c, -scaled(m, c)));
-    return scaled(m, c) < kPlainRange && s > 0.f && s < INFINITY;
+    return scaled(m, c) < kPlainRange && s >= 0.5f && s < INFINITY;
   }
 };
 

@@ -1,0 +1,95 @@
+"""Checks of the operators on logits that a NaN cannot pass: the error has to be shown small, not large."""
+
+import torch
+
+from _logits_oracle import distill, half_step, relative, score, smallest_step
+
+
+def within(got, want, room):
+    """Every value within its room of the one wanted; NaN and infinities where those are, and nowhere else."""
+    got, room = got.detach().double(), torch.as_tensor(room, device=got.device).expand(got.shape)
+    assert got.shape == want.shape and bool((room >= 0).all()) and bool(room.isfinite().all())
+    ok = torch.where(want.isnan(), got.isnan(), (got == want) | ((got - want).abs() <= room))
+    assert bool(ok.all()), (int((~ok).sum()), got[~ok][:4].tolist(), want[~ok][:4].tolist(), room[~ok][:4].tolist())
+
+
+def _rounded(grad, dtype):
+    """Infinite where the type has no such number: what lies past its largest number by half a step."""
+    past = grad.abs() > torch.finfo(dtype).max * (1 + half_step(dtype) / 2)
+    return torch.where(past, grad.sign() * float("inf"), grad)
+
+
+def check_score(logits, tokens, temperature=1.0, entropy=True, top_k=0, sums=2.0 ** -17.3):
+    """`sums`: the relative error of a row's sum.  The other bounds are those of the oracle's relative()."""
+    from fairring_b200.ops import token_log_probs
+
+    gen = torch.Generator(device=logits.device).manual_seed(1)
+    g = torch.randn(tokens.shape, device=logits.device, generator=gen)
+    h = torch.randn(tokens.shape, device=logits.device, generator=gen)
+    leaf = logits.detach().requires_grad_(True)
+    got = token_log_probs(leaf, tokens, temperature=temperature, entropy=entropy, top_k=top_k)
+    (grad,) = torch.autograd.grad([got.log_probs, got.entropy] if entropy else got.log_probs, leaf, [g, h] if entropy else g)
+    want, want_h, want_grad, logp = score(logits, tokens, temperature, g, h if entropy else None)
+    counts = tokens >= 0
+    # the difference to the maximum, the temperature, the product and the sum: 2^-24 each
+    within(got.log_probs, want, sums + 4 * 2.0 ** -24 * want.abs().where(want.isfinite(), 0.0))
+    p, far = logp.exp(), logp.clamp_min(-110).abs()
+    off = relative(logp) + sums
+    if entropy:
+        within(got.entropy, want_h, torch.where(counts, (p * (1 + far) * off).sum(-1) * 2 + sums, 0.0))
+    if top_k:
+        order = logits.float().sort(dim=-1, descending=True, stable=True).indices[..., :top_k]
+        assert torch.equal(got.top_tokens, order.where(counts.unsqueeze(-1), -1))
+        top = logp.gather(-1, order)
+        room = sums + 4 * 2.0 ** -24 * top.abs().where(top.isfinite(), 0.0)
+        within(got.top_log_probs, top.where(counts.unsqueeze(-1), float("-inf")), room)
+    size = p * (g.double().abs().unsqueeze(-1) + (h.double().abs() * (1 + want_h)).unsqueeze(-1) * (1 + far)) / temperature
+    # the type's half step; the probability; its flush to zero below 2^-126, with the factors that it meets; the 1 of the token
+    room = half_step(logits.dtype) * want_grad.abs() + 2 * off * size + smallest_step(logits.dtype)
+    room = room + 2.0 ** -126 * (g.double().abs() + 128 * h.double().abs()).unsqueeze(-1) / temperature
+    room = room + 2.0 ** -22 * g.double().abs().unsqueeze(-1) / temperature * torch.zeros_like(p).scatter_(
+        -1, tokens.clamp_min(0).unsqueeze(-1), 1.0)
+    within(grad, _rounded(want_grad, logits.dtype), torch.where(counts.unsqueeze(-1), room, 0.0))
+    return got, grad
+
+
+def check_distill(logits, tokens, given, temperature=1.0, rest=False, rows=None, sums=2.0 ** -17.4):
+    """`rows`: those of a [rows, vocab] matrix whose values are looked at."""
+    from fairring_b200.ops import distillation_loss
+
+    gen = torch.Generator(device=logits.device).manual_seed(1)
+    g = torch.randn(logits.shape[:-1], device=logits.device, generator=gen)
+    leaf = logits.detach().requires_grad_(True)
+    loss = distillation_loss(leaf, tokens, given, temperature=temperature, rest=rest, reduction="none")
+    (grad,) = torch.autograd.grad(loss, leaf, g)
+    assert loss.dtype == torch.float32 and grad.dtype == logits.dtype and grad.shape == logits.shape
+    if rows is not None:
+        logits, tokens, given, g, loss, grad = (t[rows] for t in (logits, tokens, given, g, loss.detach(), grad))
+    want, want_grad, logp = distill(logits, tokens, given, temperature, rest, g)
+    low = float("-inf")
+    there = (tokens >= 0) & ~(given == low)
+    counts = ((tokens >= 0) if rest else there).any(-1)
+    log_q = given.double() if rest else (given.double() / temperature).masked_fill(~there, low).log_softmax(-1)
+    log_q = torch.where(there & counts.unsqueeze(-1), log_q, -1e30)
+    log_p = logp.gather(-1, tokens.clamp_min(0))
+    apart = log_q.abs() + log_p.abs().where(log_p.isfinite(), 0.0) + 1
+    # A teacher's probability: an exponential (2^-22), its argument's roundings (2^-23 of it) and a sum of up to 13
+    # additions (2^-20.3), once more in what it weighs; the logarithms' own roundings; the row's sum, and the rest's.
+    q_off = 2.0 ** -19.5 + 2.0 ** -22 * log_q.abs().clamp_max(110)
+    room = (log_q.exp() * apart * (q_off + 2.0 ** -22)).sum(-1) + 2 * sums + 2.0 ** -24
+    if rest:  # what is left is the sum's rounding off, 2^-23, and weighs the logarithm of the others' share
+        listed = torch.zeros_like(logp).scatter_add_(-1, tokens.clamp_min(0), (tokens >= 0).double()) > 0
+        others = torch.logsumexp(logp.masked_fill(listed, low), -1)
+        room = room + (2.0 ** -21 + log_q.exp().sum(-1) * 2.0 ** -21) * (1 + others.abs().where(others.isfinite(), 0.0))
+    room = room + 2.0 ** -22 * want.abs().where(want.isfinite(), 0.0)
+    past = want.abs() > torch.finfo(torch.float32).max
+    within(loss, torch.where(past, want.sign() * float("inf"), want), torch.where(counts, room, 0.0))
+    p = logp.exp()
+    share, named = p, torch.zeros_like(p).scatter_add_(-1, tokens.clamp_min(0), (tokens >= 0).double()) > 0
+    if rest:  # the weight of the others' is a difference of two numbers up to 1, over their probability
+        share = p + (logp - others.unsqueeze(-1)).masked_fill(named | others.isinf().unsqueeze(-1), low).exp()
+    scale = g.double().abs().unsqueeze(-1) / temperature
+    room = half_step(logits.dtype) * want_grad.abs() + smallest_step(logits.dtype)
+    room = room + scale * (2 * (relative(logp) + sums) * share + 2.0 ** -18.5 * named + 2.0 ** -126)
+    within(grad, _rounded(want_grad, logits.dtype), torch.where(counts.unsqueeze(-1), room, 0.0))
+    return loss, grad
