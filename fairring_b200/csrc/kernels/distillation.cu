@@ -595,6 +595,7 @@ distillation_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad, cons
     float logit = 0.f;
     if (counts && (int)threadIdx.x < k) {
       mine = pairs[r * k + threadIdx.x];
+      if ((unsigned)mine.x >= (unsigned)x.vocab) mine.x = -1;  // a row that was given up has whatever the memory held
       const int v = (mine.x - parts.head) / E / (U * kThreads);
       const bool vector = mine.x >= parts.head && mine.x < parts.head + parts.nvec * E;
       if (mine.x >= 0 && (vector ? v : 0) != piece) mine.x = -1;
@@ -659,6 +660,7 @@ distillation_short_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* grad
   // The i-th listed token if it is this piece's, and its logit.
   auto listed = [&](int i, float& logit) {
     int2 pair = pairs[r * k + i];
+    if ((unsigned)pair.x >= (unsigned)x.vocab) pair.x = -1;  // as above
     const int v = (pair.x - parts.head) / E / (U * 32);
     const bool vector = pair.x >= parts.head && pair.x < parts.head + parts.nvec * E;
     if (pair.x >= 0 && (vector ? v : 0) != piece) pair.x = -1;

@@ -577,12 +577,13 @@ struct HandOver {
                  "r"(sharedAddress(&answered))
                  : "memory");
   }
-  // By a warp: the number of the block that will not start, or -1 if all have.  Waits whoever has given up: the answer comes to this
-  // block's memory.
+  // By a warp: the number of the block that will not start, -1 if all have, or kNoAnswer.  Waits whoever has given up: the answer
+  // comes to this block's memory.
+  static constexpr int kNoAnswer = -2;
   __device__ __forceinline__ int answerOf(unsigned parity) {
-    if (!barrierWait(&answered, parity)) {
+    if (!__all_sync(kAll, barrierWait(&answered, parity))) {
       *static_cast<volatile int*>(&failed) = 1;
-      return -1;
+      return kNoAnswer;
     }
     int block;
     uint32_t ok;
@@ -620,7 +621,8 @@ inline int rowsABlock(const LogitRows& x, int elem_size, int sm_count) {
 
 // The fetching warp's part.  `counts(r)`, by one lane, says that a row does not count as far as that is seen at once, else skip(r), by
 // one lane too.  prepare(r, place), by all, says for the others whether they do; mark(r, place) comes once the row's copies may begin.
-// lose(r), by one lane, leaves NaN: of every row before it is handed on, and of those that a block which gives up has taken.
+// lose(r), by one lane, leaves NaN: of every row before it is handed on, of those that a block which gives up has taken, and, where
+// that is not known since the hardware did not answer, of all: whoever has done one of them may have written it before or after.
 // Copies run kDepth - 1 batches ahead, so as many rows: nothing that a row's copies wait for may itself wait for one of the
 // kSlots - 1 rows before it.
 static_assert(kSlots >= kDepth, "a row's copies begin while the row kDepth - 1 before it is swept");
@@ -659,6 +661,8 @@ __device__ __forceinline__ void fetchRows(Counts&& counts, int64_t rows, int row
       if (mask >> lane & 1u) lose((int)mine);
       const int64_t next = (int64_t)block * rows_a_block + lane;
       if (block >= 0 && lane < rows_a_block && next < rows) lose((int)next);
+      if (block == HandOver::kNoAnswer)
+        for (int64_t r = lane; r < rows; r += 32) lose((int)r);
       return;
     }
   }

@@ -1,0 +1,60 @@
+"""How the operators on logits are called: what a program around them may have done before, between and after."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _student_and_teacher(rows, vocab, k, dtype=torch.bfloat16):
+    x = torch.randn(rows, vocab, device="cuda", generator=_gen(vocab)) * 3
+    values, tokens = (x + torch.randn(rows, vocab, device="cuda", generator=_gen(1))).log_softmax(-1).topk(k, -1)
+    return x.to(dtype), tokens, values
+
+
+# by a warp a piece, and by a block a piece
+@pytest.mark.parametrize("vocab", [1003, 16384])
+@pytest.mark.parametrize("k", [5, 40])
+def test_the_backward_of_rows_that_were_given_up(vocab, k):
+    """Such a row has NaN statistics, and where its tokens would be, whatever the memory held: its gradient is NaN, and
+    nothing else is touched."""
+    from fairring_b200.ops import distillation_loss
+
+    rows = 7
+    x, tokens, given = _student_and_teacher(rows, vocab, k)
+    lost = [1, 4, 6]
+    found = []
+
+    def give_up(t):
+        if t.dim() != 1:
+            return t
+        t = t.clone()  # 4 floats, 4 of each row, and of each row k pairs of a token's number and a probability
+        assert t.numel() == 4 + 4 * rows + 2 * k * rows
+        stats, pairs = t[4:4 + 4 * rows].view(rows, 4), t[4 + 4 * rows:].view(rows, k, 2).view(torch.int32)
+        assert torch.equal(pairs[..., 0].long(), tokens)
+        stats[lost] = float("nan")
+        held = torch.tensor([2 ** 31 - 1, vocab, -2 ** 31, -1, 0x7FC00000, vocab + 8, 3], dtype=torch.int32, device="cuda")
+        for i, r in enumerate(lost):
+            pairs[r, :, 0] = held[(torch.arange(k, device="cuda") + i) % len(held)]
+        found.append(True)
+        return t
+
+    got = []
+    for unpack in (lambda t: t, give_up):
+        leaf = x.clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            loss = distillation_loss(leaf, tokens, given, reduction="none")
+        got.append(torch.autograd.grad(loss, leaf, torch.ones(rows, device="cuda"))[0])
+    assert found
+    for r in range(rows):
+        assert bool(got[1][r].isnan().all()) if r in lost else torch.equal(got[0][r], got[1][r])
