@@ -502,6 +502,7 @@ distillation_rows_kernel(const T* __restrict__ logits, LogitRows x, Given given,
             marked_before = marked;
             marked = r;
             const unsigned loose = markListed<kThreads>(te, k, Slice<T>(row, x.vocab, 0, 1), bits, twice);
+            __syncwarp();  // every lane's marks before the arrival of one
             if (lane == 0) {
               shared.loose[at.slot] = loose;
               barrierArrive(&hand.marked[at.slot]);

@@ -746,6 +746,7 @@ __device__ __forceinline__ void sweepRows(const T* logits, const LogitRows& x, f
     }
     hook.end();
     const Sums acc = warpSums<kEntropy>(mine.sums(), c);
+    __syncwarp();  // what every lane has read of the row's slot and its marks before the arrival of one
     if ((tid & 31) == 0) {
       out.sums[at.slot][tid >> 5] = acc;
       barrierArrive(&out.full[at.slot]);
