@@ -728,8 +728,10 @@ cudaError_t forwardOf(const T* logits, const LogitRows& x, const DistillationArg
   }
   const int slices = slicesFor(x.rows, x.vocab, sizeof(T), sm_count);
   const size_t shared = 4 * (kNameWords + (kRest ? Marks<T>::words((x.vocab / Vec<T>::kElems + slices - 1) / slices) : 0));
-  if (shared > 32 * 1024)
-    cudaFuncSetAttribute(distillation_slices_kernel<T, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+  if (shared > 32 * 1024) {
+    const cudaError_t e = allowShared(reinterpret_cast<const void*>(&distillation_slices_kernel<T, kRest>), shared);
+    if (e != cudaSuccess) return e;
+  }
   return launchSlices(distillation_slices_kernel<T, kRest>, x.rows, slices, kSliceThreads, shared, stream, logits, x, given, c, inv_t, loss,
                       stats, pairs);
 }
@@ -757,13 +759,11 @@ cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const
   // 8192 x 8200 52.8 -> 45.8; but 8192 x 16384, which fills the blocks, 77 -> 86, and 4000 fp32 logits 36 -> 40.
   Pieces warps;
   if (warps.template cut<T>(x) && warps.a_row <= 16 && (int)warps.a_row < 6 * pieces)
-    distillation_short_bwd_kernel<T><<<warps.blocks(), kThreads, 0, stream>>>(static_cast<const T*>(logits), x, static_cast<T*>(grad), st,
-                                                                              listed, k, c, inv_t, upstream, stride, count, warps);
-  else
-    distillation_bwd_kernel<T><<<(unsigned)(total < (1 << 30) ? total : (1 << 30)), kThreads, 0, stream>>>(
-        static_cast<const T*>(logits), x, static_cast<T*>(grad), st, listed, k, c, inv_t, upstream, stride, count, total, pieces);
-  noteLocalLaunch();
-  return cudaGetLastError();
+    return launchBlocks(distillation_short_bwd_kernel<T>, warps.blocks(), kThreads, 1, 0, stream, static_cast<const T*>(logits), x,
+                        static_cast<T*>(grad), st, listed, k, c, inv_t, upstream, stride, count, warps);
+  return launchBlocks(distillation_bwd_kernel<T>, (unsigned)(total < (1 << 30) ? total : (1 << 30)), kThreads, 1, 0, stream,
+                      static_cast<const T*>(logits), x, static_cast<T*>(grad), st, listed, k, c, inv_t, upstream, stride, count, total,
+                      pieces);
 }
 
 }  // namespace
@@ -782,9 +782,7 @@ cudaError_t launchDistillation(const void* logits, const LogitRows& x, const Dis
 
 cudaError_t launchDistillationMean(const float* loss, const float* stats, int64_t rows, float* mean, float* count,
                                    cudaStream_t stream) {
-  distillation_mean_kernel<<<1, 1024, 0, stream>>>(loss, reinterpret_cast<const float4*>(stats), rows, mean, count);
-  noteLocalLaunch();
-  return cudaGetLastError();
+  return launchBlocks(distillation_mean_kernel, 1, 1024, 1, 0, stream, loss, reinterpret_cast<const float4*>(stats), rows, mean, count);
 }
 
 cudaError_t launchDistillationBackward(const void* logits, const LogitRows& x, void* grad, const float* stats,

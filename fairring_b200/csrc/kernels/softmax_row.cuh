@@ -29,6 +29,9 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #include "local_kernels.h"
 
@@ -461,23 +464,50 @@ inline int slicesFor(int64_t rows, int vocab, int elem_size, int sm_count) {
   return n;
 }
 
+// The status is the launch's own: cudaGetLastError() would also return, and clear, an error that the host program has pending from
+// something else.
+inline cudaError_t ownStatus(cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();  // reported here, so not once more by whoever asks next
+  return e;
+}
 template <typename... Params, typename... Args>
-cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, int threads, size_t shared, cudaStream_t stream,
+cudaError_t launchBlocks(void (*kernel)(Params...), unsigned blocks, int threads, int cluster, size_t shared, cudaStream_t stream,
                          Args... args) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(rows * slices));
+  config.gridDim = dim3(blocks);
   config.blockDim = dim3((unsigned)threads);
   config.dynamicSmemBytes = shared;
   config.stream = stream;
   cudaLaunchAttribute attribute = {};
   attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = (unsigned)slices;
+  attribute.val.clusterDim.x = (unsigned)cluster;
   attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
   config.attrs = &attribute;
-  config.numAttrs = slices > 1 ? 1 : 0;
-  cudaLaunchKernelEx(&config, kernel, Params(args)...);
-  noteLocalLaunch();
-  return cudaGetLastError();
+  config.numAttrs = cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, Params(args)...);
+  if (e == cudaSuccess) noteLocalLaunch();
+  return ownStatus(e);
+}
+// Lets a kernel's launches have that much shared memory.  Said once for a kernel, a device and a size, since saying it clears the
+// error that may be pending, and never less than before: another thread may be about to launch with that.
+inline cudaError_t allowShared(const void* kernel, size_t bytes) {
+  static std::mutex mutex;
+  static std::map<std::pair<const void*, int>, size_t> allowed;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return ownStatus(e);
+  const std::lock_guard<std::mutex> lock(mutex);
+  size_t& most = allowed[{kernel, device}];
+  if (bytes <= most) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) most = bytes;
+  return ownStatus(e);
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, int threads, size_t shared, cudaStream_t stream,
+                         Args... args) {
+  return launchBlocks(kernel, (unsigned)(rows * slices), threads, slices, shared, stream, args...);
 }
 
 // ---- many rows -----------------------------------------------------------------
@@ -768,10 +798,9 @@ template <class Finish> __device__ __forceinline__ void finishRows(HandOver& out
 
 template <typename... Params, typename... Args>
 cudaError_t launchRows(void (*kernel)(Params...), int64_t rows, int rows_a_block, size_t shared, cudaStream_t stream, Args... args) {
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-  kernel<<<(unsigned)((rows + rows_a_block - 1) / rows_a_block), kRowThreads, shared, stream>>>(Params(args)...);
-  noteLocalLaunch();
-  return cudaGetLastError();
+  const cudaError_t e = allowShared(reinterpret_cast<const void*>(kernel), shared);
+  if (e != cudaSuccess) return e;
+  return launchBlocks(kernel, (unsigned)((rows + rows_a_block - 1) / rows_a_block), kRowThreads, 1, shared, stream, args...);
 }
 
 // Whether rows are many enough for that: several for each of the blocks that stay.
@@ -789,9 +818,7 @@ inline bool shortRows(const LogitRows& x, int elem_size, int sm_count) {
 }
 template <typename... Params, typename... Args>
 cudaError_t launchShort(void (*kernel)(Params...), int64_t rows, size_t shared, cudaStream_t stream, Args... args) {
-  kernel<<<(unsigned)((rows + kWarps - 1) / kWarps), kThreads, shared, stream>>>(Params(args)...);
-  noteLocalLaunch();
-  return cudaGetLastError();
+  return launchBlocks(kernel, (unsigned)((rows + kWarps - 1) / kWarps), kThreads, 1, shared, stream, args...);
 }
 
 }  // namespace softmax_row

@@ -729,11 +729,9 @@ cudaError_t backwardOf(const void* logits, const LogitRows& x, void* grad, const
   if (!pieces.template cut<T>(x)) return cudaErrorInvalidValue;
   const float inv_t = (float)(1.0 / a.temperature), c = (float)(1.4426950408889634 / a.temperature);
   auto run = [&](auto kernel) {
-    kernel<<<pieces.blocks(), kThreads, 0, stream>>>(static_cast<const T*>(logits), x, static_cast<T*>(grad), a.tokens,
-                                            reinterpret_cast<const float2*>(a.stats), a.entropy, a.g_log_probs, a.g_stride,
-                                            a.g_entropy, a.h_stride, c, inv_t, pieces);
-    noteLocalLaunch();
-    return cudaGetLastError();
+    return launchBlocks(kernel, pieces.blocks(), kThreads, 1, 0, stream, static_cast<const T*>(logits), x, static_cast<T*>(grad), a.tokens,
+                        reinterpret_cast<const float2*>(a.stats), a.entropy, a.g_log_probs, a.g_stride, a.g_entropy, a.h_stride, c,
+                        inv_t, pieces);
   };
   return a.g_entropy != nullptr ? run(token_log_probs_bwd_kernel<T, true>) : run(token_log_probs_bwd_kernel<T, false>);
 }

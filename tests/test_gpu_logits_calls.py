@@ -1,5 +1,7 @@
 """How the operators on logits are called: what a program around them may have done before, between and after."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -58,3 +60,32 @@ def test_the_backward_of_rows_that_were_given_up(vocab, k):
     assert found
     for r in range(rows):
         assert bool(got[1][r].isnan().all()) if r in lost else torch.equal(got[0][r], got[1][r])
+
+
+# the forms of the forward: slices of a cluster, a block with more shared memory than a launch has by itself, blocks that stay, a
+# warp a row
+@pytest.mark.parametrize("rows,vocab", [(3, 20011), (160, 300001), (700, 20011), (700, 1003)])
+def test_an_error_that_the_host_has_pending(rows, vocab):
+    """It is neither reported by these calls nor cleared."""
+    from fairring_b200.ops import distillation_loss, token_log_probs
+
+    x, tokens, given = _student_and_teacher(rows, vocab, 5)
+    first = tokens[:, 0].contiguous()
+    runtime = ctypes.CDLL("libcudart.so.12")  # the one that torch and the package use
+
+    def calls():
+        yield from token_log_probs(x, first, entropy=True)[:2]
+        yield from token_log_probs(x, first, top_k=4)[2:]
+        for rest in (False, True):
+            yield distillation_loss(x, tokens, given, rest=rest)
+
+    want = list(calls())
+    torch.cuda.synchronize()
+    refused = runtime.cudaSetDevice(4096)  # no such device: an error of the host call alone
+    assert refused != 0
+    try:
+        got = list(calls())
+    finally:
+        pending = runtime.cudaGetLastError()
+    assert pending == refused
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
