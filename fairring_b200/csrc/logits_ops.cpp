@@ -153,26 +153,28 @@ TokenLogProbs tokenLogProbsForward(const Rows& rows, const std::optional<at::Ten
 // The gradient of the logits from torch's ops, where its own graph is wanted.
 at::Tensor tokenLogProbsBackwardGraph(const at::Tensor& logits, const at::Tensor& tokens, double temperature,
                                       const at::Tensor& g_log_probs, const at::Tensor& g_entropy) {
-  at::Tensor counts, wide = logits.to(at::kFloat);
+  at::Tensor counts, known, wide = logits.to(at::kFloat);
   if (tokens.defined()) {  // a row that does not count is not looked at, be it NaN
     counts = tokens.ge(0).unsqueeze(-1);
+    known = counts.logical_and(tokens.lt(logits.size(-1)).unsqueeze(-1));
     wide = wide.masked_fill(counts.logical_not(), 0.0);
   }
   const at::Tensor logp = at::log_softmax(wide / temperature, -1), p = logp.exp();
   at::Tensor grad = at::zeros_like(p);
   if (g_log_probs.defined()) {
-    const at::Tensor known = tokens.ge(0).logical_and(tokens.lt(logits.size(-1))).unsqueeze(-1);
     const at::Tensor at = tokens.unsqueeze(-1).where(known, at::zeros_like(tokens).unsqueeze(-1));
     const at::Tensor g = g_log_probs.unsqueeze(-1);
     grad = (at::zeros_like(p).scatter_(-1, at, 1.0) - p) * g;
-    grad = grad.masked_fill(counts.logical_and(known.logical_not()), std::numeric_limits<double>::quiet_NaN());
   }
   if (g_entropy.defined()) {
     const at::Tensor finite = logp.masked_fill(p.eq(0), 0.0);
     const at::Tensor h = -(p * finite).sum(-1, true);
     grad = grad - p * (finite + h) * g_entropy.unsqueeze(-1);
   }
-  if (counts.defined()) grad = at::where(counts, grad, at::zeros_like(grad));
+  if (counts.defined()) {
+    grad = grad.masked_fill(known.logical_not(), std::numeric_limits<double>::quiet_NaN());
+    grad = at::where(counts, grad, at::zeros_like(grad));
+  }
   return (grad / temperature).to(logits.scalar_type());
 }
 

@@ -58,8 +58,9 @@ def token_log_probs(logits: torch.Tensor, tokens: torch.Tensor | None = None, *,
 
     A negative token (-100) marks a row that does not count: log probability and entropy 0, its
     ``top_tokens`` -1 at minus infinity, its gradient 0, and its logits are not looked at.  A token past the
-    vocabulary has the log probability NaN, and the row's gradient is NaN.  Logits of minus infinity have probability 0; a
-    row of nothing else, or with a NaN or infinite one, gives NaN as ``log_softmax`` does.  ``log_probs`` and
+    vocabulary has the log probability NaN, and the row's gradient is NaN, whichever output it is of.  Logits of
+    minus infinity have probability 0; a row of nothing else, or with a NaN or infinite one, gives NaN as
+    ``log_softmax`` does.  ``log_probs`` and
     ``entropy`` carry gradients to the logits, the largest entries are for reading.
 
     On the GPU the leading dimensions may have any order and strides (a batch without its last position,
@@ -86,11 +87,15 @@ def _plain_token_log_probs(logits, tokens, temperature, entropy, top_k) -> Token
     of = h = top = which = None
     if tokens is not None:
         known = counts & (tokens < logits.shape[-1])
+        unknown = counts & ~known
         of = logp.gather(-1, tokens.where(known, 0).unsqueeze(-1)).squeeze(-1)
-        of = torch.where(counts, of, 0.0) * torch.where(counts & ~known, float("nan"), 1.0)
+        of = torch.where(counts, of, 0.0) * torch.where(unknown, float("nan"), 1.0)
     if entropy:
         h = -(logp.exp() * logp.masked_fill(logp == float("-inf"), 0.0)).sum(-1)
-        h = h if counts is None else torch.where(counts, h, 0.0)
+        if counts is not None:
+            h = torch.where(counts, h, 0.0)
+            # The row's gradient is NaN though the entropy is not: 0 times the slope of a root at zero.
+            h = h + 0.0 * torch.where(unknown, h - h.detach(), 1.0).sqrt()
     if top_k:
         order = wide.detach().sort(dim=-1, descending=True, stable=True).indices[..., :top_k]
         top, which = logp.detach().gather(-1, order), order

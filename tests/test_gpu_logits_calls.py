@@ -89,3 +89,24 @@ def test_an_error_that_the_host_has_pending(rows, vocab):
         pending = runtime.cudaGetLastError()
     assert pending == refused
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_entropys_gradient_past_the_vocabulary(dtype):
+    """NaN by the kernel, by the backward that has a graph and by torch's operations, whichever output is used."""
+    from fairring_b200.ops.token_log_probs import _plain_token_log_probs, token_log_probs
+
+    x = _student_and_teacher(4, 1003, 1, dtype)[0]
+    tokens = torch.tensor([5, 1003, -100, 2 ** 40], device="cuda")
+    for used in (lambda o: o.entropy.sum(), lambda o: o.log_probs.sum(), lambda o: o.entropy.sum() + o.log_probs.sum()):
+        grads = []
+        for call, graph in ((token_log_probs, False), (token_log_probs, True),
+                            (lambda z, t, entropy: _plain_token_log_probs(z, t, 1.0, entropy, 0), False)):
+            leaf = x.clone().requires_grad_(True)
+            out = call(leaf, tokens, entropy=True)
+            assert bool(out.entropy.isfinite().all())
+            grads.append(torch.autograd.grad(used(out), leaf, create_graph=graph)[0].detach())
+        for grad in grads:
+            assert bool(grad[1].isnan().all()) and bool(grad[3].isnan().all()) and not grad[2].any()
+            # A probability is 2^-20 of itself off, and p |log p| + p H is below 7.4: both sides 2^-17.1, and a rounding to the type.
+            torch.testing.assert_close(grad[0], grads[0][0], rtol=torch.finfo(dtype).eps + 2.0 ** -19, atol=2.0 ** -16)

@@ -139,3 +139,19 @@ def test_what_looks_through_them():
         assert loss.shape == () and loss.dtype == torch.float32 and loss.device.type == "cuda"
     slope = torch.func.grad(lambda z: token_log_probs(z, t).log_probs.sum())(x)
     torch.testing.assert_close(slope, score(x, t, g=torch.ones(3))[2].float(), rtol=1e-5, atol=1e-6)
+
+
+def test_the_entropys_gradient_past_the_vocabulary():
+    """NaN as the log probability's, though the entropy itself is known; twice, where the gradient has a graph."""
+    x, tokens = _logits(3, 7), torch.tensor([6, 7, -1])
+    for graph in (False, True):
+        leaf = x.clone().requires_grad_(True)
+        got = token_log_probs(leaf, tokens, entropy=True)
+        want, want_grad = score(x, tokens.clamp_max(6), h=torch.ones(3))[1:3]
+        torch.testing.assert_close(got.entropy.double(), want, rtol=1e-6, atol=2e-6)
+        (grad,) = torch.autograd.grad(got.entropy.sum(), leaf, create_graph=graph)
+        assert bool(grad[1].isnan().all()) and not grad[2].any()
+        torch.testing.assert_close(grad[0].double(), want_grad[0], rtol=1e-6, atol=2e-6)
+        if graph:
+            (second,) = torch.autograd.grad((grad[0] ** 2).sum(), leaf)
+            assert bool(second[0].isfinite().all()) and bool(second[0].any())
