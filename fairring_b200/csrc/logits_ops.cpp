@@ -315,7 +315,9 @@ at::Tensor distillationBackwardGraph(const at::Tensor& logits, const at::Tensor&
     const at::Tensor mass = q.to(at::kDouble).sum(-1, true), some = 1 - mass;
     const at::Tensor left = at::where(some.ge(kLeastRest), some, at::zeros_like(some));
     const at::Tensor listed = at::zeros_like(z).scatter_add_(-1, at, known.to(z.scalar_type())).gt(0);
-    const at::Tensor share = at::softmax(z.masked_fill(listed, low), -1).masked_fill(listed, 0.0);
+    const at::Tensor gone = listed.logical_or(z.eq(low)).all(-1, true);  // no other token has any probability
+    const at::Tensor share =
+        at::softmax(z.masked_fill(listed.logical_and(gone.logical_not()), low), -1).masked_fill(listed.logical_or(gone), 0.0);
     grad = grad * (mass + left).to(at::kFloat) - at::where(left.gt(0), share * left.to(at::kFloat), at::zeros_like(share));
   } else {
     q = at::softmax((log_probs / temperature).masked_fill(known.logical_not(), low), -1).masked_fill(known.logical_not(), 0.0);

@@ -76,9 +76,11 @@ def _plain_distillation(logits, tokens, given, temperature, rest):
         left = 1 - q.double().sum(-1)
         left = torch.where(left >= _C.LEAST_REST, left, 0.0)
         listed = torch.zeros_like(logp).scatter_add_(-1, at, known.to(logp.dtype)) > 0
-        # A row whose every token is listed has no other: its sum is over nothing, and so is its gradient.
-        empty = listed.all(-1, keepdim=True)
-        others = torch.logsumexp(logp.masked_fill(listed & ~empty, low), -1).masked_fill(empty.squeeze(-1), low)
+        # No other token, or none with any probability: the loss is infinite, and the gradient that of the row's own sum.
+        gone = (listed | (logp == low)).all(-1, keepdim=True)
+        others = torch.logsumexp(logp.masked_fill(listed & ~gone, low), -1)
+        less_sum = (logp - wide / temperature).gather(-1, logp.detach().argmax(-1, keepdim=True)).squeeze(-1)
+        others = torch.where(gone.squeeze(-1), low + (less_sum - less_sum.detach()), others)
         share = left * (left.clamp_min(1e-300).log() - others.double())
         loss = loss + torch.where(left > 0, share, 0.0).to(loss.dtype)
     loss = loss * torch.where((there & ~known).any(-1), float("nan"), 1.0)

@@ -110,3 +110,26 @@ def test_the_entropys_gradient_past_the_vocabulary(dtype):
             assert bool(grad[1].isnan().all()) and bool(grad[3].isnan().all()) and not grad[2].any()
             # A probability is 2^-20 of itself off, and p |log p| + p H is below 7.4: both sides 2^-17.1, and a rounding to the type.
             torch.testing.assert_close(grad[0], grads[0][0], rtol=torch.finfo(dtype).eps + 2.0 ** -19, atol=2.0 ** -16)
+
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_a_rest_without_probability(temperature):
+    """The same by the kernel, by the backward that has a graph and by torch's operations; second derivatives too."""
+    from fairring_b200.ops import distillation_loss
+    from fairring_b200.ops.distillation import _plain_distillation
+    from test_logits_ops import _without_others
+
+    x, tokens, given, want = (t.cuda() for t in _without_others())
+    grads, seconds = [], []
+    for native, graph in ((True, False), (True, True), (False, True)):
+        leaf = (x * temperature).requires_grad_(True)
+        loss = (distillation_loss(leaf, tokens, given, temperature=temperature, rest=True, reduction="none") if native
+                else _plain_distillation(leaf, tokens, given, temperature, True)[0])
+        assert loss.isinf().tolist() == [True, True, False, False]
+        (grad,) = torch.autograd.grad(loss.sum(), leaf, create_graph=graph)
+        # a probability's 2^-17, and a few roundings of numbers up to 1
+        torch.testing.assert_close(grad.double(), want / temperature, rtol=2.0 ** -16, atol=2.0 ** -20)
+        if graph:
+            seconds.append(torch.autograd.grad((grad ** 2).sum(), leaf)[0])
+    assert bool(seconds[0].isfinite().all())
+    torch.testing.assert_close(*seconds, rtol=1e-4, atol=1e-6)

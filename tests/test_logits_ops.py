@@ -155,3 +155,33 @@ def test_the_entropys_gradient_past_the_vocabulary():
         if graph:
             (second,) = torch.autograd.grad((grad[0] ** 2).sum(), leaf)
             assert bool(second[0].isfinite().all()) and bool(second[0].any())
+
+
+def _without_others():
+    """Rows of 12 logits whose every other token is masked, with every token listed, with a single other one, and
+    with one that the teacher gives nothing; the distributions' parts of 0.9."""
+    x = _logits(4, 12, seed=3)
+    tokens = torch.arange(12).expand(4, 12).clone()
+    tokens[0, 3:], tokens[2, 11], tokens[3, 5:] = -1, -1, -1
+    x[0, 3:] = float("-inf")
+    x[3, 8:] = float("-inf")
+    given = (torch.linspace(-2, 0, 12).expand(4, 12).masked_fill(tokens < 0, float("-inf")).log_softmax(-1) - 0.105).where(tokens >= 0, -3.0)
+    p, q = x.double().softmax(-1), torch.zeros(4, 12, dtype=torch.float64)
+    q.scatter_add_(1, tokens.clamp_min(0), given.double().exp().where(tokens >= 0, 0.0))
+    for r in (0, 1):  # rows 2 and 3 are the oracle's
+        assert not distill(x[r:r + 1], tokens[r:r + 1], given[r:r + 1], rest=True)[0].isfinite()
+    want = torch.cat([(p - q)[:2], distill(x[2:], tokens[2:], given[2:], rest=True)[1]])
+    return x, tokens, given, want
+
+
+def test_a_rest_without_probability():
+    """The loss is infinite, and the gradient that of the row's sum alone, Q p - q with Q = 1, as from the kernel."""
+    x, tokens, given, want = _without_others()
+    for graph in (False, True):
+        leaf = x.clone().requires_grad_(True)
+        loss = distillation_loss(leaf, tokens, given, rest=True, reduction="none")
+        assert loss.isinf().tolist() == [True, True, False, False]
+        (grad,) = torch.autograd.grad(loss.sum(), leaf, create_graph=graph)
+        torch.testing.assert_close(grad.double(), want, rtol=1e-5, atol=1e-6)
+        if graph:
+            assert bool(torch.autograd.grad((grad ** 2).sum(), leaf)[0].isfinite().all())
