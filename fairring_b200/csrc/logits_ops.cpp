@@ -320,7 +320,9 @@ at::Tensor distillationBackwardGraph(const at::Tensor& logits, const at::Tensor&
         at::softmax(z.masked_fill(listed.logical_and(gone.logical_not()), low), -1).masked_fill(listed.logical_or(gone), 0.0);
     grad = grad * (mass + left).to(at::kFloat) - at::where(left.gt(0), share * left.to(at::kFloat), at::zeros_like(share));
   } else {
-    q = at::softmax((log_probs / temperature).masked_fill(known.logical_not(), low), -1).masked_fill(known.logical_not(), 0.0);
+    // A row without any mass does not count; its softmax is NaN, which a factor of zero would hand on.
+    const at::Tensor none = known.logical_not().logical_or(counts.logical_not());
+    q = at::softmax((log_probs / temperature).masked_fill(known.logical_not(), low), -1).masked_fill(none, 0.0);
   }
   grad = grad.scatter_add(-1, at, -q);
   grad = grad.masked_fill(bad, std::numeric_limits<double>::quiet_NaN());

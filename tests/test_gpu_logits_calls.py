@@ -133,3 +133,28 @@ def test_a_rest_without_probability(temperature):
             seconds.append(torch.autograd.grad((grad ** 2).sum(), leaf)[0])
     assert bool(seconds[0].isfinite().all())
     torch.testing.assert_close(*seconds, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_second_derivative_past_a_teacher_without_mass(rest, reduction):
+    """Listed tokens of minus infinity: without the rest the row does not count, and its derivatives are 0."""
+    from fairring_b200.ops import distillation_loss
+    from fairring_b200.ops.distillation import _plain_distillation
+
+    x, tokens, given = _student_and_teacher(4, 33, 6, torch.float32)
+    given = given - 0.1
+    given[1], given[2, 1:] = float("-inf"), float("-inf")
+    got = []
+    for native in (True, False):
+        leaf = x.clone().requires_grad_(True)
+        if native:
+            loss = distillation_loss(leaf, tokens, given, rest=rest, reduction=reduction)
+        else:
+            loss, counts = _plain_distillation(leaf, tokens, given, 1.0, rest)
+            loss = loss.sum() / counts.sum() if reduction == "mean" else loss
+        (g,) = torch.autograd.grad((loss ** 2).sum(), leaf, create_graph=True)
+        got.append([g, torch.autograd.grad((g ** 2).sum(), leaf)[0]])
+    for a, b in zip(*got):
+        assert bool(a.isfinite().all()) and bool(a[1].any()) == rest
+        torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6)
