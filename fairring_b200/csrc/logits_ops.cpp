@@ -108,6 +108,9 @@ std::tuple<at::Tensor, int64_t> perRow(const at::Tensor& g) {
   return std::make_tuple(t.contiguous(), 1);
 }
 
+// Saved-tensor hooks may have brought it back in another layout.
+at::Tensor dense(const at::Tensor& saved) { return saved.defined() ? saved.contiguous() : saved; }
+
 // int64, contiguous, from integers of that shape on the logits' device.
 at::Tensor checkTokens(const at::Tensor& tokens, const at::Tensor& logits, at::IntArrayRef sizes, const char* name) {
   TORCH_CHECK_VALUE(at::isIntegralType(tokens.scalar_type(), false), name, " must be integers, not ", tokens.scalar_type());
@@ -198,7 +201,7 @@ struct TokenLogProbsNode : torch::autograd::Function<TokenLogProbsNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &logits = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
+    const at::Tensor &logits = saved[0], tokens = dense(saved[1]), stats = dense(saved[2]), entropy = dense(saved[3]);
     const double temperature = ctx->saved_data["temperature"].toDouble();
     at::Tensor g, h;
     size_t i = 0;
@@ -343,18 +346,18 @@ struct DistillationNode : torch::autograd::Function<DistillationNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &logits = saved[0], none;
+    const at::Tensor &logits = saved[0], memory = dense(saved[3]), none;
     const double temperature = ctx->saved_data["temperature"].toDouble();
     const bool mean = ctx->saved_data["mean"].toBool();
     if (at::GradMode::is_enabled())
       return {distillationBackwardGraph(logits, saved[1], saved[2], temperature, ctx->saved_data["rest"].toBool(), mean, grads[0],
-                                        saved[3]),
+                                        memory),
               none, none, none, none, none};
     c10::cuda::CUDAGuard guard(logits.device());
     Rows rows = rowsOf(logits);
     const at::Tensor grad = gradientFor(rows);
     const auto [g, stride] = perRow(grads[0]);
-    const Kept kept(saved[3], rows.x.rows);
+    const Kept kept(memory, rows.x.rows);
     const cudaError_t e = launchDistillationBackward(rows.t.data_ptr(), rows.x, grad.data_ptr(), kept.stats, kept.pairs,
                                                      (int)saved[1].size(-1), temperature, g.data_ptr<float>(), stride,
                                                      mean ? kept.count : nullptr, c10::cuda::getCurrentCUDAStream());

@@ -158,3 +158,33 @@ def test_second_derivative_past_a_teacher_without_mass(rest, reduction):
     for a, b in zip(*got):
         assert bool(a.isfinite().all()) and bool(a[1].any()) == rest
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-6)
+
+
+def _other_layout(t):
+    """The same values, the last dimension no longer the one without gaps."""
+    return t if t.dim() < 2 else t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize("hooks", ["pinned", "pageable", "another layout"])
+@pytest.mark.parametrize("rest", [False, True])
+def test_saved_tensors_that_come_back_in_another_layout(hooks, rest):
+    from fairring_b200.ops import distillation_loss, token_log_probs
+
+    x, tokens, given = (t.view(4, 9, -1) for t in _student_and_teacher(36, 1003, 5))
+    first = tokens[..., 0].clone()
+    first[1, 3] = -100
+
+    def grads():
+        leaf = x.clone().requires_grad_(True)
+        with hook:
+            out = token_log_probs(leaf, first, entropy=True)
+            loss = distillation_loss(leaf, tokens, given, rest=rest)
+        up = torch.randn(2, 4, 9, device="cuda", generator=_gen(3))
+        return [*torch.autograd.grad([out.log_probs, out.entropy], leaf, list(up)), *torch.autograd.grad(loss, leaf)]
+
+    hook = torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t)
+    want = grads()
+    hook = (torch.autograd.graph.saved_tensors_hooks(lambda t: t, _other_layout) if hooks == "another layout"
+            else torch.autograd.graph.save_on_cpu(pin_memory=hooks == "pinned"))
+    for a, b in zip(grads(), want):
+        assert torch.equal(a, b)
