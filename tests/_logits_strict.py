@@ -19,8 +19,9 @@ def _rounded(grad, dtype):
     return torch.where(past, grad.sign() * float("inf"), grad)
 
 
-def check_score(logits, tokens, temperature=1.0, entropy=True, top_k=0, sums=2.0 ** -17.3):
-    """`sums`: the relative error of a row's sum.  The other bounds are those of the oracle's relative()."""
+def check_score(logits, tokens, temperature=1.0, entropy=True, top_k=0, rows=None, sums=2.0 ** -17.3):
+    """`rows`: those of a [rows, vocab] matrix whose values are looked at.  `sums`: the relative error of a row's sum.  The other
+    bounds are those of the oracle's relative()."""
     from fairring_b200.ops import token_log_probs
 
     gen = torch.Generator(device=logits.device).manual_seed(1)
@@ -29,6 +30,9 @@ def check_score(logits, tokens, temperature=1.0, entropy=True, top_k=0, sums=2.0
     leaf = logits.detach().requires_grad_(True)
     got = token_log_probs(leaf, tokens, temperature=temperature, entropy=entropy, top_k=top_k)
     (grad,) = torch.autograd.grad([got.log_probs, got.entropy] if entropy else got.log_probs, leaf, [g, h] if entropy else g)
+    if rows is not None:
+        got = type(got)(*(v if v is None else v.detach()[rows] for v in got))
+        logits, tokens, g, h, grad = (t[rows] for t in (logits, tokens, g, h, grad))
     want, want_h, want_grad, logp = score(logits, tokens, temperature, g, h if entropy else None)
     counts = tokens >= 0
     # the difference to the maximum, the temperature, the product and the sum: 2^-24 each

@@ -61,3 +61,40 @@ def test_distillation_at_the_end_of_the_fast_exponent(rows, vocab, scale, rest):
         near = (torch.arange(rows, device="cuda") % 2 == 0).view(-1, 1)
         x.scatter_(1, tokens, torch.where(near, x.gather(1, tokens) + 726880.0 * scale, x.gather(1, tokens)))
     check_distill(x, tokens, given if rest else given * scale, scale, rest)
+
+
+def _equal_but_one(rows, vocab, dtype, top, step):
+    """Every logit `step` below `top`, but for one in what each thread of a block sees first: then the exponentials are no powers
+    of two, and each addition of one to a sum rounds the same way."""
+    x = torch.full((rows, vocab), top - step, device="cuda", dtype=dtype)
+    each = 16 // x.element_size()
+    x[:, : 256 * each: each] = top
+    return x
+
+
+# What a sum of V logits may be off: 16 additions of a batch's and one for each of V / 4096 batches (32 values of 16 bits or 16 of 32
+# a thread of 256, by one block), 23 that merge and rescale; 2^-24 each.
+def _sums(vocab):
+    return (16 + vocab / 4096 + 23) * 2.0 ** -24
+
+
+# eight slices a row, two, blocks that stay
+@pytest.mark.parametrize("rows", [1, 160, 600])
+@pytest.mark.parametrize("kind", ["equal", "spread"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_million_columns(rows, kind, dtype):
+    vocab = (1 << 20) + (5 if kind == "spread" else 0)
+    x = (_equal_but_one(rows, vocab, dtype, 0.0, 5.625) if kind == "equal" else
+         (torch.randn(rows, vocab, device="cuda", generator=_gen(1)) * 3).to(dtype))
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(2))
+    some = torch.tensor([0, rows // 2, rows - 1], device="cuda")
+    check_score(x, tokens, rows=some, sums=_sums(vocab))
+    check_score(x, tokens, entropy=False, rows=some, sums=_sums(vocab))
+
+
+# by a block, and by a warp, whose lanes would round 2^15 times
+@pytest.mark.parametrize("rows", [1, 600])
+def test_a_million_columns_that_are_looked_at_again(rows):
+    x = _equal_but_one(rows, 1 << 20, torch.float32, -3e6, 2.5)
+    tokens = torch.randint(0, 1 << 20, (rows,), device="cuda", generator=_gen(2))
+    check_score(x, tokens, rows=torch.tensor([0, rows - 1], device="cuda"), sums=40 * 2.0 ** -24)
