@@ -534,7 +534,9 @@ constexpr int kManyRows = 4;  // for each multiprocessor: 700 rows of 32003 fp32
 constexpr int kDepth = 3;     // two batches of 16 KB on their way for each of the three blocks; one more gained nothing
 constexpr int kRowThreads = kThreads + 64;  // sweep, then the warp that fetches, then the one that finishes
 constexpr int kSlots = 3;                   // rows between being fetched and being finished; 4 to 6: 134 -> 136 us, with the rest 155 -> 171
-constexpr uint64_t kPatience = 4000000000ull;  // nanoseconds after which a wait is given up
+constexpr uint32_t kPatience = 4000000000u;  // nanoseconds after which a wait is given up,
+constexpr uint32_t kMostStep = 10000000u;    // and those that count of any one try
+static_assert(kPatience + kMostStep > kPatience, "what has been waited does not start again");
 
 __device__ __forceinline__ uint32_t sharedAddress(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void barrierInit(uint64_t* bar, int arrivals) {
@@ -552,16 +554,22 @@ __device__ __forceinline__ bool barrierTry(uint64_t* bar, unsigned parity) {
       : "memory");
   return done != 0;
 }
-__device__ __forceinline__ uint64_t nanoseconds() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+__device__ __forceinline__ uint32_t nanoseconds() {  // modulo 2^32
+  uint32_t t;
+  asm volatile("mov.u32 %0, %globaltimer_lo;" : "=r"(t));
   return t;
 }
+// False if the wait is given up.  What a block waits for is done by its own warps, so a block that was stopped (by a debugger, or
+// for another context) finds it as it was: that time is no reason to give up.
 __device__ __forceinline__ bool barrierWait(uint64_t* bar, unsigned parity) {
   if (barrierTry(bar, parity)) return true;
-  const uint64_t start = nanoseconds();
-  while (!barrierTry(bar, parity))
-    if (nanoseconds() - start > kPatience) return false;
+  uint32_t waited = 0, before = nanoseconds();
+  while (!barrierTry(bar, parity)) {
+    const uint32_t now = nanoseconds();
+    waited += min(now - before, kMostStep);
+    before = now;
+    if (waited > kPatience) return false;
+  }
   return true;
 }
 __device__ __forceinline__ void copyAhead(uint4* to, const uint4* from) {
