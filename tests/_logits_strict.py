@@ -2,7 +2,7 @@
 
 import torch
 
-from _logits_oracle import distill, half_step, relative, score, smallest_step
+from _logits_oracle import half_step, relative, score, smallest_step
 
 
 def within(got, want, room):
@@ -57,6 +57,49 @@ def check_score(logits, tokens, temperature=1.0, entropy=True, top_k=0, rows=Non
     return got, grad
 
 
+def distill_by_formula(logits, tokens, given, temperature=1.0, rest=False, g=None):
+    """(loss of every row, gradient of sum(g * loss), log-softmax, logarithm of the others' share), in 64 bits.  Beside logits of
+    1e16 and more a logarithm is lost even there, so every sum is of differences to its own largest value."""
+    low = float("-inf")
+    x, given = logits.detach().double(), given.detach().double()
+    there = tokens >= 0
+    at = tokens.clamp_min(0)
+    counts = (there if rest else there & (given != low)).any(-1)
+
+    def log_sum(z):
+        top = z.amax(-1, keepdim=True)
+        return top, ((z - top) / temperature).exp().sum(-1, keepdim=True).log()
+
+    top, log_s = log_sum(x)
+    logp = (x - top) / temperature - log_s
+    p = logp.exp()
+    if rest:
+        log_q = given.masked_fill(~there, low)
+    else:
+        log_q = (given / temperature).masked_fill(~(there & counts.unsqueeze(-1)), low).log_softmax(-1)
+        log_q = log_q.masked_fill(~there, low)
+    q = torch.where(there & counts.unsqueeze(-1), log_q.exp(), 0.0)
+    loss = torch.where(q > 0, q * (log_q - logp.gather(-1, at)), 0.0).sum(-1)
+    q_of = torch.zeros_like(p).scatter_add_(-1, at, q)
+    mass, log_rest = q.sum(-1, keepdim=True), None
+    grad = p * mass - q_of
+    if rest:
+        left = 1 - mass
+        left = left.where(left >= 2.0 ** -20, 0.0)  # less is the rounding of the teacher's values
+        listed = torch.zeros_like(p).scatter_add_(-1, at, there.double()) > 0
+        others = x.masked_fill(listed, low)
+        top_o, log_o = log_sum(others)
+        none = top_o == low
+        log_rest = torch.where(none, low, (top_o - top) / temperature + log_o - log_s)
+        share = torch.where(none | listed, 0.0, ((others - top_o) / temperature - log_o).exp())
+        loss = loss + torch.where(left > 0, left * (left.log() - log_rest), 0.0).squeeze(-1)
+        grad = torch.where(listed, p * (mass + left) - q_of, share * ((mass + left) * log_rest.exp() - left))
+        log_rest = log_rest.squeeze(-1)
+    up = 1.0 if g is None else g.double().unsqueeze(-1)
+    grad = torch.where(counts.unsqueeze(-1), grad * up / temperature, 0.0)
+    return torch.where(counts, loss, 0.0), grad, logp, log_rest
+
+
 def check_distill(logits, tokens, given, temperature=1.0, rest=False, rows=None, sums=2.0 ** -17.4):
     """`rows`: those of a [rows, vocab] matrix whose values are looked at."""
     from fairring_b200.ops import distillation_loss
@@ -69,7 +112,7 @@ def check_distill(logits, tokens, given, temperature=1.0, rest=False, rows=None,
     assert loss.dtype == torch.float32 and grad.dtype == logits.dtype and grad.shape == logits.shape
     if rows is not None:
         logits, tokens, given, g, loss, grad = (t[rows] for t in (logits, tokens, given, g, loss.detach(), grad))
-    want, want_grad, logp = distill(logits, tokens, given, temperature, rest, g)
+    want, want_grad, logp, others = distill_by_formula(logits, tokens, given, temperature, rest, g)
     low = float("-inf")
     there = (tokens >= 0) & ~(given == low)
     counts = ((tokens >= 0) if rest else there).any(-1)
@@ -82,8 +125,6 @@ def check_distill(logits, tokens, given, temperature=1.0, rest=False, rows=None,
     q_off = 2.0 ** -19.5 + 2.0 ** -22 * log_q.abs().clamp_max(110)
     room = (log_q.exp() * apart * (q_off + 2.0 ** -22)).sum(-1) + 2 * sums + 2.0 ** -24
     if rest:  # what is left is the sum's rounding off, 2^-23, and weighs the logarithm of the others' share
-        listed = torch.zeros_like(logp).scatter_add_(-1, tokens.clamp_min(0), (tokens >= 0).double()) > 0
-        others = torch.logsumexp(logp.masked_fill(listed, low), -1)
         room = room + (2.0 ** -21 + log_q.exp().sum(-1) * 2.0 ** -21) * (1 + others.abs().where(others.isfinite(), 0.0))
     room = room + 2.0 ** -22 * want.abs().where(want.isfinite(), 0.0)
     past = want.abs() > torch.finfo(torch.float32).max
@@ -91,7 +132,8 @@ def check_distill(logits, tokens, given, temperature=1.0, rest=False, rows=None,
     p = logp.exp()
     share, named = p, torch.zeros_like(p).scatter_add_(-1, tokens.clamp_min(0), (tokens >= 0).double()) > 0
     if rest:  # the weight of the others' is a difference of two numbers up to 1, over their probability
-        share = p + (logp - others.unsqueeze(-1)).masked_fill(named | others.isinf().unsqueeze(-1), low).exp()
+        x = logits.double().masked_fill(named, low)
+        share = p + ((x - x.amax(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).min)) / temperature).softmax(-1).nan_to_num(0.0)
     scale = g.double().abs().unsqueeze(-1) / temperature
     room = half_step(logits.dtype) * want_grad.abs() + smallest_step(logits.dtype)
     room = room + scale * (2 * (relative(logp) + sums) * share + 2.0 ** -18.5 * named + 2.0 ** -126)

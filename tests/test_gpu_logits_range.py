@@ -5,8 +5,11 @@ import pytest
 import torch
 
 from _logits_strict import check_distill, check_score
+from test_gpu_distillation import _case
 
 pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
 @pytest.fixture(autouse=True)
@@ -81,7 +84,7 @@ def _sums(vocab):
 # eight slices a row, two, blocks that stay
 @pytest.mark.parametrize("rows", [1, 160, 600])
 @pytest.mark.parametrize("kind", ["equal", "spread"])
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_a_million_columns(rows, kind, dtype):
     vocab = (1 << 20) + (5 if kind == "spread" else 0)
     x = (_equal_but_one(rows, vocab, dtype, 0.0, 5.625) if kind == "equal" else
@@ -98,3 +101,96 @@ def test_a_million_columns_that_are_looked_at_again(rows):
     x = _equal_but_one(rows, 1 << 20, torch.float32, -3e6, 2.5)
     tokens = torch.randint(0, 1 << 20, (rows,), device="cuda", generator=_gen(2))
     check_score(x, tokens, rows=torch.tensor([0, rows - 1], device="cuda"), sums=40 * 2.0 ** -24)
+
+
+# ---- what the other tests of these operators look at too, with checks that a NaN cannot pass ----------------------------
+def _logits(rows, vocab, dtype, seed=0):
+    x = torch.randn(rows, vocab, device="cuda", generator=_gen(seed + vocab)) * 3
+    x[:, vocab // 2] += 6
+    return x.to(dtype)
+
+
+def _tokens(rows, vocab):
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(vocab))
+    if rows > 5:
+        tokens[3], tokens[4], tokens[5] = -100, 0, vocab - 1
+    return tokens
+
+
+@pytest.mark.parametrize("rows", [1, 19, 400, 1300])
+@pytest.mark.parametrize("vocab", [1, 7, 9, 1001, 4096, 8193, 16385, 32776])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_of_every_form(rows, vocab, dtype):
+    x, tokens = _logits(rows, vocab, dtype), _tokens(rows, vocab)
+    check_score(x, tokens, 0.7, top_k=min(vocab, 5))
+    check_score(x, tokens, entropy=False)
+
+
+@pytest.mark.parametrize("rows", [1, 19, 400, 1300])
+@pytest.mark.parametrize("vocab,k", [(2, 1), (7, 3), (1001, 256), (8193, 64), (16385, 33), (32776, 5)])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_of_every_form(rows, vocab, k, rest, dtype):
+    x, tokens, given = _case(rows, vocab, k, dtype)
+    check_distill(x, tokens, given - 0.2 if rest else given, 1.3, rest)
+
+
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 1e6])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probs_at_extreme_temperatures(rows, vocab, temperature, dtype):
+    x, tokens = _logits(rows, vocab, dtype), _tokens(rows, vocab)
+    tokens[6::3] = x[6::3].float().argmax(-1)
+    check_score(x, tokens, temperature, top_k=5)
+
+
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 1e6])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_at_extreme_temperatures(rows, vocab, temperature, rest, dtype):
+    """The teacher is as sharp as the student, or with the rest is what it is."""
+    x, tokens, given = _case(rows, vocab, 20, dtype)
+    check_distill(x, tokens, given * 1.2 - 0.1 if rest else given, temperature, rest)
+
+
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_of_values_that_are_no_numbers(rows, vocab, rest, dtype):
+    """NaN and infinity, listed or not, make their own row NaN and no other; a row that does not count may hold anything."""
+    from fairring_b200.ops import distillation_loss
+
+    x, tokens, given = _case(rows, vocab, 9, dtype, padded=0.0)
+    given = given * 1.2 - 0.1 if rest else given
+    tokens[4:6], bad = -1, x.clone()
+    listed = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda").scatter_(1, tokens.clamp_min(0), True)
+    bad[0, int((~listed[0]).nonzero()[7])] = float("nan")
+    bad[1, int((~listed[1]).nonzero()[-1])] = float("inf")
+    bad[6, tokens[6, 2]], bad[3, tokens[3, 4]] = float("nan"), float("inf")
+    bad[4], bad[5, 0] = float("nan"), float("inf")
+    got = []
+    for z in (x, bad):
+        leaf = z.clone().requires_grad_(True)
+        loss = distillation_loss(leaf, tokens, given, rest=rest, reduction="none")
+        got.append((loss.detach(), torch.autograd.grad(loss, leaf, torch.ones(rows, device="cuda"))[0]))
+    broken = [0, 1, 3, 6]
+    fine = torch.ones(rows, dtype=torch.bool, device="cuda")
+    fine[broken] = False
+    for a, b in zip(*got):
+        assert bool(b[broken].isnan().all()) and bool(a.isfinite().all())
+        assert torch.equal(a[fine], b[fine]) and not b[4:6].any()
+
+
+# slices with more shared memory than a launch has by itself; a block a row where blocks that stay would hold too many marks;
+# the widest
+@pytest.mark.parametrize("rows,vocab", [(5, 1 << 20), (160, 520_001), (600, 220_001), (600, 1 << 20)])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distillation_over_wide_vocabularies(rows, vocab, rest, dtype):
+    x = torch.randn(rows, vocab, device="cuda", generator=_gen(vocab)).mul_(3).to(dtype)
+    tokens = torch.randint(0, vocab, (rows, 64), device="cuda", generator=_gen(1))
+    tokens[:, 3], tokens[:, 4], tokens[1, 9], tokens[0, 7] = 0, vocab - 1, tokens[1, 8], -1
+    given = torch.randn(rows, 64, device="cuda", generator=_gen(2)).log_softmax(-1) - 0.105
+    x.scatter_add_(1, tokens.clamp_min(0), torch.full((rows, 64), 6.0, device="cuda", dtype=dtype))
+    check_distill(x, tokens, given, 1.0, rest, rows=torch.tensor([0, 1, rows // 2, rows - 1], device="cuda"), sums=_sums(vocab))

@@ -8,6 +8,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from _logits_oracle import distill, score
+from _logits_strict import distill_by_formula, within
 from fairring_b200.ops import distillation_loss, token_log_probs
 
 
@@ -185,3 +186,36 @@ def test_a_rest_without_probability():
         torch.testing.assert_close(grad.double(), want, rtol=1e-5, atol=1e-6)
         if graph:
             assert bool(torch.autograd.grad((grad ** 2).sum(), leaf)[0].isfinite().all())
+
+
+def test_the_strict_check_sees_what_is_no_number():
+    """A NaN or an infinity where the oracle has a number, or the other way round, does not pass, whatever the room."""
+    value, room = torch.tensor([1.0, -2.0, 3.0]), torch.tensor([0.1, 0.1, 0.1])
+    within(value, value.double(), room)
+    within(value, value.double() + 0.09, room)
+    odd = torch.tensor([1.0, float("nan"), float("-inf")])
+    within(odd, odd.double(), room)
+    for other in (float("nan"), float("inf"), 1.11):
+        for swapped in (False, True):
+            wrong = value.clone()
+            wrong[0] = other
+            with pytest.raises(AssertionError):
+                within(*((value, wrong.double()) if swapped else (wrong, value.double())), room)
+    for no_room in (float("nan"), float("inf"), -1.0):
+        with pytest.raises(AssertionError):
+            within(value, value.double(), torch.tensor([0.1, no_room, 0.1]))
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 2.5])
+def test_the_formula_against_the_definition(rest, temperature):
+    """The closed form of the loss's gradient in 64 bits against autograd's of the definition."""
+    x = _logits(7, 23, seed=5)
+    x[6, 15:] = float("-inf")
+    tokens = torch.tensor([[0, 22, 3, 7], [1, 1, 2, 1], [-1, -1, -1, -1], [5, -100, 6, 8], [9, 8, 7, 22], [4, 4, 4, 4], [3, 2, 1, 0]])
+    given = torch.log(torch.tensor([0.3, 0.25, 0.2, 0.1])).expand(7, 4).clone()
+    given[4, 1], g = float("-inf"), torch.linspace(-1, 2, 7)
+    want, want_grad, want_logp = distill(x, tokens, given, temperature, rest, g)
+    loss, grad, logp, _ = distill_by_formula(x, tokens, given, temperature, rest, g)
+    for a, b in ((loss, want), (grad, want_grad), (logp[:2], want_logp[:2])):
+        torch.testing.assert_close(a, b, rtol=1e-12, atol=1e-12)
