@@ -254,14 +254,15 @@ __device__ __forceinline__ void finishRow(const Listed& l, const Sums& acc, bool
     above = acc.s == 0.f ? 0.f : exp2Of((acc.m - m) * c);
     s = acc.s * above + (l.s == 0.f ? 0.f : l.s * exp2Of((l.m - m) * c));
   }
-  const double lse = (double)m * inv_t + log((double)s), mass = l.mass;
+  // Differences are taken before the temperature and the logarithm come in: beside logits of 2^53 and more a logarithm is nothing.
+  const double log_s = log((double)s), mass = l.mass;
   double sum = l.log_terms - l.from_ref * inv_t;
-  if (!(mass == 0)) sum -= mass * (log((double)l.total) + (double)l.ref * inv_t - lse);
+  if (!(mass == 0)) sum -= mass * (log((double)l.total) + (((double)l.ref - m) * inv_t - log_s));
   const float nan = __int_as_float(0x7fffffff);
   float4 st = make_float4(m, 1.f / s, m, 1.f / s);
   if constexpr (kRest) {
     const double q_rest = 1.0 - mass < kLeastRest ? 0.0 : 1.0 - mass;  // NaN stays
-    if (!(q_rest == 0)) sum += q_rest * (log(q_rest) - ((double)acc.m * inv_t + log((double)acc.s) - lse));
+    if (!(q_rest == 0)) sum += q_rest * (log(q_rest) - (((double)acc.m - m) * inv_t + (log((double)acc.s) - log_s)));
     const double all = mass + q_rest, p_rest = (double)(acc.s * above) / s;
     const bool some = !(acc.s == 0.f);
     st = make_float4(some ? acc.m : 0.f, some ? (float)((all * p_rest - q_rest) / acc.s) : 0.f, m, (float)(all / s));

@@ -155,6 +155,40 @@ def test_distillation_at_extreme_temperatures(rows, vocab, temperature, rest, dt
 
 
 @pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("shift", [3e6, -3e6, 1e30, -1e30])
+@pytest.mark.parametrize("rest", [False, True])
+def test_distillation_far_from_zero(rows, vocab, shift, rest):
+    """Every row, every other row, and of every other row what is not listed or only that."""
+    base, tokens, given = _case(rows, vocab, 9, torch.float32, padded=0.0)
+    given = given * 1.2 - 0.1 if rest else given
+    listed = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda").scatter_(1, tokens.clamp_min(0), True)
+    odd = (torch.arange(rows, device="cuda") % 2 == 1).view(-1, 1)
+    for where in (torch.ones_like(odd), odd, odd & ~listed, odd & listed):
+        check_distill(torch.where(where, base + shift, base), tokens, given, 1.0, rest)
+
+
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_distillation_of_masked_logits(rows, vocab, rest, dtype):
+    """Minus infinity and the type's lowest value, up to all that is not listed and whole rows."""
+    lowest = torch.finfo(dtype).min
+    for fill in (float("-inf"), lowest):
+        x, tokens, given = _case(rows, vocab, 9, dtype)
+        given = given * 1.2 - 0.1 if rest else given
+        listed = torch.zeros(rows, vocab, dtype=torch.bool, device="cuda").scatter_(1, tokens.clamp_min(0), True)
+        gone = torch.rand(rows, vocab, device="cuda", generator=_gen(3)) < 0.9
+        gone[1] = True
+        gone[1, vocab - 1] = False  # a single one left that is not listed
+        gone[3, : vocab - 30] = True  # whole slices without one
+        gone &= ~listed
+        gone[:, 5] &= fill == lowest  # with the rest, of minus infinity the loss would be infinite
+        if fill == lowest:
+            gone[4], x[5] = ~listed[4], lowest
+        check_distill(x.masked_fill(gone, fill), tokens, given, 1.0, rest)
+
+
+@pytest.mark.parametrize("rows,vocab", FORMS)
 @pytest.mark.parametrize("rest", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_distillation_of_values_that_are_no_numbers(rows, vocab, rest, dtype):
