@@ -228,3 +228,16 @@ def test_distillation_over_wide_vocabularies(rows, vocab, rest, dtype):
     given = torch.randn(rows, 64, device="cuda", generator=_gen(2)).log_softmax(-1) - 0.105
     x.scatter_add_(1, tokens.clamp_min(0), torch.full((rows, 64), 6.0, device="cuda", dtype=dtype))
     check_distill(x, tokens, given, 1.0, rest, rows=torch.tensor([0, 1, rows // 2, rows - 1], device="cuda"), sums=_sums(vocab))
+
+
+# blocks that stay, a block a row where there are largest entries or marks too many, a warp a row
+@pytest.mark.parametrize("rows,vocab", [(2100, 1 << 20), (2_200_003, 1001)])
+def test_rows_past_two_to_the_31_elements(rows, vocab):
+    x = torch.empty(rows, vocab, device="cuda", dtype=torch.bfloat16).normal_(0, 3, generator=_gen(1))
+    some = torch.tensor([0, 1, rows // 2, rows - 2, rows - 1], device="cuda")
+    check_score(x, torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(2)), top_k=9, rows=some, sums=_sums(vocab))
+    check_score(x, torch.randint(0, vocab, (rows,), device="cuda", generator=_gen(2)), entropy=False, rows=some, sums=_sums(vocab))
+    tokens = torch.randint(0, vocab, (rows, 6), device="cuda", generator=_gen(3))
+    given = torch.randn(rows, 6, device="cuda", generator=_gen(4)).log_softmax(-1) - 0.2
+    for rest in (False, True):
+        check_distill(x, tokens, given, 1.0, rest, rows=some, sums=_sums(vocab))
