@@ -8,9 +8,11 @@
 //   dx_v = 1/T (Q p_v - q_v) for a listed token, 1/T (p_v / p_r) (Q p_r - q_r) for any other.
 // p_r is summed from the tokens that are not listed: 1 - sum p_k would lose it where the teacher's tokens are likely.
 //
-// Forward one read of the logits, backward one read and one write; the listed tokens' own logits are read apart, and their
-// gradients written over those of the sweep.  8192 x 51200 bf16, 64 tokens: forward 140 to 147 us, backward 254 (6.6 TB/s; both together
-// 391 us at the copy rate); 2 x 1024 x 51200 with the rest 48 and 61 (91).
+// Forward one read of the logits, backward one read and one write; the listed tokens' own logits
+// are read apart, and their gradients written over those of the sweep.  8192 x 51200 bf16, 64
+// tokens: forward 139 us, 149 while the last gradient is still written back from L2, backward 254
+// (6.6 TB/s; both together 391 us at the copy rate); 2 x 1024 x 51200 with the rest 45 or 48 and 61
+// (91).
 #include "softmax_row.cuh"
 
 namespace fairring {

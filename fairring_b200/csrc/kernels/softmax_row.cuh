@@ -7,20 +7,24 @@
 // order of the slices; many by blocks that stay and take row after row; many short ones by a warp each.  Which it is depends on
 // the sizes alone, and so does the order of every sum.
 //
-// What bounds it: the bytes, and next to them the exponentials (16 a clock and multiprocessor: 9 TB/s of bf16 logits) and the
-// instructions around them.  8192 rows of 51200 bf16 logits: 134 us, 6.3 TB/s; 61 instructions of a warp for 32 vectors of 8, of them 9
-// for the special function unit, 21 for the multiply-add pipe, 19 integer and comparisons, 4 loads and stores; 60 % of the issue
-// slots.  fp32 logits need half of that a byte: 2 x 1023 rows of 50265 in 65 us, 6.3 TB/s.  So the instructions are kept few: no
-// comparison of the maximum a value but one a batch, in the logits' own type; two fp32 operations in one instruction (157 us at the
-// time, 164 without); no test for what masked rows need.  A polynomial in place of some exponentials costs more issue slots than
-// it frees (157 -> 178).
+// What bounds it: the bytes, and next to them the exponentials (16 a clock and multiprocessor: 9
+// TB/s of bf16 logits) and the instructions around them.  8192 rows of 51200 bf16 logits: 132 us,
+// 6.4 TB/s; 61 instructions of a warp for 32 vectors of 8, of them 9 for the special function unit,
+// 23 for the multiply-add pipe, 18 integer and comparisons, 4 loads and stores; 60 % of the issue
+// slots.  fp32 logits need half of that a byte: 2046 rows of 50265 in 70 us, 5.9 TB/s, 6 us above
+// the copy rate.  So the instructions are kept few: no comparison of the maximum a value but one a
+// batch, in the logits' own type; two fp32 operations in one instruction (157 us at the time, 164
+// without); no test for what masked rows need.  A polynomial in place of some exponentials costs
+// more issue slots than it frees (157 -> 178).
 //
-// exp() is 2^((x - m) * c) with c = log2(e) / T, as one fused multiply-add of x, c and the rounded m * c; what that
-// rounding changes all exponentials by is put right at the row's end.  The exponential's own error is 2^-22 of a
-// probability.  That form needs |m * c| < 2^20.  A thread's m starts at -2^20 / c.  A row whose largest value is above has a sum of 1 or
-// more, but for roundings.  One whose largest value is below (masked with the type's lowest value or with minus infinity throughout,
-// say) has lost its smaller values to zero, and all of them from 126 / c below on: its sum is smaller than 1/2 unless it has lost nothing
-// that fp32 sees, and it is looked at again, slowly, as are rows above that range and those with a NaN.
+// exp() is 2^((x - m) * c) with c = log2(e) / T, as one fused multiply-add of x, c and the rounded
+// m * c; what that rounding changes all exponentials by is put right at the row's end.  The
+// exponential's own error is 2^-22 of a probability.  That form needs |m * c| < 2^20.  A thread's m
+// starts at -2^20 / c.  A row whose largest value is above has a sum of 1 or more, but for
+// roundings.  One whose largest value is below (masked with the type's lowest value or with minus
+// infinity throughout, say) has lost its smaller values to zero, and all of them from 126 / c below
+// on: its sum is smaller than 1/2 unless it has lost nothing that fp32 sees, and it is looked at
+// again, slowly, as are rows above that range and those with a NaN.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -230,10 +234,11 @@ struct Sums {
   }
 };
 
-// A thread's share of a row, from the first of its vectors on.  A batch is summed by itself and then added: a sum of V logits is 16 + V / 4096
-// additions long at most in place of V / 512, each 2^-24 off.  Rows of 2^20 equal logits but for one a thread came out 3e-5 off and are
-// now 1e-6; 8192 x 51200 bf16 takes 132 us either way.  The running sums are single numbers, since pairs spilled registers
-// where the entropy and largest entries are asked for (191 -> 203 us).
+// A thread's share of a row, from the first of its vectors on.  A batch is summed by itself and
+// then added: a sum of V logits is 16 + V / 4096 additions long at most in place of V / 512, each
+// 2^-24 off.  Rows of 2^20 equal logits but for one a thread came out 3e-5 off and are now 1e-6;
+// 8192 x 51200 bf16 takes 132 us either way.  The running sums are single numbers, since pairs
+// spilled registers where the entropy and largest entries are asked for (191 -> 203 us).
 struct ThreadSums {
   float m, at;  // at = m * c
   float s, a;
@@ -530,6 +535,9 @@ cudaError_t launchSlices(void (*kernel)(Params...), int64_t rows, int slices, in
 //  - eight warps sweep: every thread copies its own vectors to shared memory, kDepth - 1 batches ahead and
 //    across the ends of rows, and waits for its own copies alone;
 //  - one warp finishes rows while the next ones are swept.
+// Read alone, 51200 bf16 logits a row, us and above the copy rate: 592 rows 19.6 (10.2), 1000 23.9
+// (8.0), 2048 41.5 (9.0), 4096 71.8 (6.7), 8192 132.1 (1.9): the start, and the last rows of each
+// block.
 constexpr int kManyRows = 4;  // for each multiprocessor: 700 rows of 32003 fp32 logits 25.5 us by a block each, 21.5 here; 515 even, 300 the other way
 constexpr int kDepth = 3;     // two batches of 16 KB on their way for each of the three blocks; one more gained nothing
 constexpr int kRowThreads = kThreads + 64;  // sweep, then the warp that fetches, then the one that finishes

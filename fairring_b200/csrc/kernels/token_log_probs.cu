@@ -4,9 +4,9 @@
 // With z = x / T, m and S of softmax_row.cuh:  log p_v = (z_v - max z) - log S,  H = log S - A ln 2 / S, a sum of two
 // terms that are not negative.  Backward:  dx_v = 1/T [ g (1[v = t] - p_v) - h p_v (log p_v + H) ].
 //
-// Forward one read of the logits, backward one read and one write.  4 x 1024 x 51200 bf16 with the entropy, a quarter of the rows
-// not counting: forward 68 us, backward 121 (6.1 TB/s; both together 163 us at the copy rate); 8192 x 51200 with
-// the 64 largest entries 188 us (131 at the copy rate).
+// Forward one read of the logits, backward one read and one write.  4 x 1024 x 51200 bf16 with the
+// entropy, a quarter of the rows not counting: forward 68 us, backward 120 (6.1 TB/s; both together
+// 163 us at the copy rate); 8192 x 51200 with the 64 largest entries 188 us (131 at the copy rate).
 #include <cfloat>
 #include <cmath>
 
@@ -627,9 +627,12 @@ token_log_probs_rows_kernel(const T* __restrict__ logits, LogitRows x, Outputs o
   });
 }
 
-// A warp does one batch of vectors of one row, so that all are alike whatever the vocabulary; a block a batch of 16 KB left threads
-// idle at the row's end: 4 x 1024 x 51200 125 -> 121 us, 8192 x 8200 bf16 58 -> 44, 8192 x 1000 22 -> 7.  Six blocks a
-// multiprocessor (40 registers); with the 56 that it would take without the entropy 8192 x 20000 fp32 took 210 us and now takes 185.
+// A warp does one batch of vectors of one row, so that all are alike whatever the vocabulary; a
+// block a batch of 16 KB left threads idle at the row's end: 4 x 1024 x 51200 125 -> 121 us, 8192 x
+// 8200 bf16 58 -> 44, 8192 x 1000 22 -> 7.  Six blocks a multiprocessor (40 registers, of which
+// types of 16 bits spill three, one with the entropy); with five (48, no spills) 8192 x 20000 fp32
+// takes 190 us for 187, 4096 x 51200 fp16 126 for 123, 8192 x 51200 bf16 247 for 246, 8192 x 1000
+// bf16 5.7 for 6.5, all without the entropy.
 template <typename T, bool kEntropy>
 __global__ void __launch_bounds__(kThreads, 6)
 token_log_probs_bwd_kernel(const T* __restrict__ logits, LogitRows x, T* __restrict__ grad,
