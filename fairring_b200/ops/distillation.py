@@ -24,7 +24,8 @@ def distillation_loss(logits: torch.Tensor, teacher_tokens: torch.Tensor, teache
     ``rest=True``: the listed values are log probabilities over the whole vocabulary, taken at this temperature, and
     what they leave of 1 is the probability of "any other token", of the teacher as of the student:
     ``sum_k q_k (log q_k - log p_k) + q_rest (log q_rest - log p_rest)``.  Less than 2^-20 is what rounding leaves of
-    values that sum to 1, and counts as nothing.
+    values that sum to 1, and counts as nothing.  Where the teacher leaves more and the student nothing (every other token
+    is masked or listed) the loss is infinite.
 
     A negative token is padding.  A row of padding (or, without the rest, of nothing but values of minus infinity) does
     not count: its loss and gradient are 0.  A token named twice is two terms of the sum, and one token of the
