@@ -368,25 +368,39 @@ __device__ __forceinline__ Sums scan(const Slice<T>& sl, float c, Hook& hook) {
   return acc.sums();
 }
 
-// Two sweeps over a row for what the fast one cannot do, by `size` threads: this one's share of it, relative to m.  Summed in 64 bits:
-// a warp that does a whole row of 2^20 logits adds 2^15 to each sum.
+// Two sweeps over a row for what the fast one cannot do, by `warps` warps: the largest value, and this
+// lane's share of the sums, relative to it.  A warp takes 1024 columns at once, of which a lane has every
+// 32nd; leave.of(base), by all lanes, has a bit for each of the lane's that is to be left out.  Summed
+// in 64 bits: a warp that does a whole row of 2^20 logits adds 2^15 to each sum.
+constexpr unsigned kChunk = 1024;
+template <typename T, class Leave, class Take>
+__device__ __forceinline__ void eachAgain(const T* row, int vocab, int warp, int warps,
+                                          const Leave& leave, Take&& take) {
+  for (unsigned base = warp * kChunk; base < (unsigned)vocab; base += warps * kChunk) {
+    const unsigned out = leave.of(base);
+#pragma unroll 16
+    for (unsigned j = 0; j < 32; ++j) {
+      const unsigned col = base + 32 * j + (threadIdx.x & 31);
+      take(col < (unsigned)vocab && !(out >> j & 1u) ? toFloat(row[col]) : -INFINITY);
+    }
+  }
+}
 template <typename T, bool kEntropy, class Leave>
-__device__ __noinline__ Sums lookAgain(const T* row, int vocab, int rank, int size, float c, float top, Leave leave) {
+__device__ __noinline__ Sums lookAgain(const T* row, int vocab, int warp, int warps, float c,
+                                       float top, Leave leave) {
   const float ref = top == -INFINITY ? 0.f : top;
   double s = 0, a = 0;
-  for (int col = rank; col < vocab; col += size) {
-    if (leave(col)) continue;
-    const float d = (toFloat(row[col]) - ref) * c, e = exp2Of(d);
+  eachAgain(row, vocab, warp, warps, leave, [&](float v) {
+    const float d = (v - ref) * c, e = exp2Of(d);
     s += e;
     if (kEntropy) a += e * fmaxf(d, kLowExponent);
-  }
+  });
   return {top, (float)s, (float)a};
 }
 template <typename T, class Leave>
-__device__ __noinline__ float largestOf(const T* row, int vocab, int rank, int size, Leave leave) {
+__device__ __noinline__ float largestOf(const T* row, int vocab, int warp, int warps, Leave leave) {
   float top = -INFINITY;
-  for (int col = rank; col < vocab; col += size)
-    if (!leave(col)) top = fmaxf(top, toFloat(row[col]));
+  eachAgain(row, vocab, warp, warps, leave, [&](float v) { top = fmaxf(top, v); });
   return top;
 }
 
@@ -424,13 +438,13 @@ template <bool kEntropy> __device__ __forceinline__ Sums blockSums(Sums acc, flo
 // A row's sums, relative to m, by a whole block, its first kThreads threads, or a whole warp, where the sweep's did not settle.
 template <typename T, bool kEntropy, class Leave>
 __device__ __noinline__ Sums blockAgain(const T* row, int vocab, float c, Sums* scratch, Leave leave) {
-  const int mine = threadIdx.x < kThreads ? vocab : 0;
-  float top = warpMax(largestOf(row, mine, (int)threadIdx.x, kThreads, leave));
+  const int mine = threadIdx.x < kThreads ? vocab : 0, warp = threadIdx.x >> 5;
+  float top = warpMax(largestOf(row, mine, warp, kWarps, leave));
   __syncthreads();
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5].m = top;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) top = fmaxf(top, scratch[i].m);
-  Sums acc = lookAgain<T, kEntropy>(row, mine, (int)threadIdx.x, kThreads, c, top, leave);
+  Sums acc = lookAgain<T, kEntropy>(row, mine, warp, kWarps, c, top, leave);
   acc.s = warpSum(acc.s);
   acc.a = warpSum(acc.a);
   __syncthreads();
@@ -442,15 +456,14 @@ __device__ __noinline__ Sums blockAgain(const T* row, int vocab, float c, Sums* 
 }
 template <typename T, bool kEntropy, class Leave>
 __device__ __noinline__ Sums warpAgain(const T* row, int vocab, float c, Leave leave) {
-  const int lane = threadIdx.x & 31;
-  const float top = warpMax(largestOf(row, vocab, lane, 32, leave));
-  Sums acc = lookAgain<T, kEntropy>(row, vocab, lane, 32, c, top, leave);
+  const float top = warpMax(largestOf(row, vocab, 0, 1, leave));
+  Sums acc = lookAgain<T, kEntropy>(row, vocab, 0, 1, c, top, leave);
   acc.s = warpSum(acc.s);
   acc.a = warpSum(acc.a);
   return acc;
 }
 struct LeaveNone {
-  __device__ __forceinline__ bool operator()(int) const { return false; }
+  __device__ __forceinline__ unsigned of(unsigned) const { return 0; }
 };
 
 // The row's sums from those of the slices' blocks, in the threads of block 0.  Every block of the cluster calls

@@ -188,3 +188,34 @@ def test_saved_tensors_that_come_back_in_another_layout(hooks, rest):
             else torch.autograd.graph.save_on_cpu(pin_memory=hooks == "pinned"))
     for a, b in zip(grads(), want):
         assert torch.equal(a, b)
+
+
+def _device_time(call, repeat=5):
+    """The least of some runs' microseconds, by events."""
+    call()
+    times = []
+    for _ in range(repeat):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        call()
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end) * 1000)
+    return min(times)
+
+
+# by a block, by one warp of those that stay, by a warp a row
+@pytest.mark.parametrize("rows,vocab", [(40, 51200), (700, 51200), (1400, 8000)])
+@pytest.mark.parametrize("fill", [float("-inf"), torch.finfo(torch.bfloat16).min])
+def test_a_rest_that_is_masked_takes_no_longer_with_more_listed(rows, vocab, fill):
+    """Students that may say nothing but what their teacher lists are looked at again, row by row.  That was done with a look
+    through the listed tokens for every logit: 28 times as long with 256 of them as with four."""
+    from fairring_b200.ops import distillation_loss
+
+    x, tokens, given = _student_and_teacher(rows, vocab, 256)
+    x = torch.full_like(x, fill).scatter_(1, tokens, x.gather(1, tokens))
+    few = torch.where(torch.arange(256, device="cuda") < 4, tokens, -1)
+    masked = torch.full_like(x, fill).scatter_(1, tokens[:, :4], x.gather(1, tokens[:, :4]))
+    times = [_device_time(lambda: distillation_loss(z, t.contiguous(), given[:, : t.shape[1]].contiguous(), rest=True, reduction="none"))
+             for z, t in ((masked, few[:, :4]), (x, tokens))]
+    assert times[1] <= 8 * times[0], times
